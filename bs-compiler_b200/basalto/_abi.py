@@ -16,7 +16,8 @@ MAX_TAPS = 2304
 MAX_TERMS = 2304
 
 BST_OK, BST_ERR_INVALID, BST_ERR_UNSUPPORTED, BST_ERR_CUDA, BST_ERR_NCCL, BST_ERR_TIMEOUT, BST_ERR_NO_DEVICE = range(7)
-BST_F32, BST_F64 = 0, 1
+BST_F32, BST_F64, BST_BF16, BST_F16 = range(4)
+BST_SCAN_FORWARD, BST_SCAN_BACKWARD, BST_SCAN_SAVED = range(3)
 BST_PROGRAM_CONTRACT = 1  # program flag: fold later multiplied terms with fma
 TERM_SUM, TERM_MUL, TERM_DIV = 0, 1, 2
 BOUNDARY_ZERO, BOUNDARY_VALID = 0, 1
@@ -54,6 +55,25 @@ class CDeviceCaps(ctypes.Structure):
         ("driver", ctypes.c_char * 32),
         ("driver_version", c_int32),
     ]
+
+
+class CNormDesc(ctypes.Structure):
+    _fields_ = ([(k, c_int32) for k in ("dtype", "param_dtype")]
+                + [(k, c_int64) for k in ("rows", "dim", "x_row", "y_row", "dy_row", "dx_row")] + [("eps", c_double)])
+
+
+class CConvDesc(ctypes.Structure):
+    _fields_ = ([(k, c_int32) for k in ("dtype", "param_dtype", "width", "silu", "lines")]
+                + [(k, c_int64) for k in ("batch", "length", "channels", "x_batch", "x_step", "y_batch", "y_step",
+                                          "dy_batch", "dy_step", "dx_batch", "dx_step")])
+
+
+class CScanDesc(ctypes.Structure):
+    _fields_ = ([(k, c_int32) for k in ("dtype", "softplus")]
+                + [(k, c_int64) for k in ("batch", "length", "channels", "states", "groups", "u_batch", "u_step",
+                                          "delta_batch", "delta_step", "z_batch", "z_step", "y_batch", "y_step",
+                                          "dy_batch", "dy_step", "B_batch", "B_step", "B_group", "C_batch", "C_step",
+                                          "C_group")])
 
 
 # (name, restype, argtypes) for every entry point of include/basalto_b200.h
@@ -110,6 +130,19 @@ SIGNATURES = [
     ("bst_comm_profile_begin", c_int32, [c_void_p, c_int32]),
     ("bst_march_item_plan", c_int32, [c_int64, c_int64, c_int32, c_int32, c_int64, POINTER(c_int64)]),
     ("bst_comm_profile_end", c_int32, [c_void_p, POINTER(c_double)]),
+    ("bst_layer_norm_forward", c_int32, [POINTER(CNormDesc)] + [c_void_p] * 7),
+    ("bst_layer_norm_workspace", c_int32, [POINTER(CNormDesc), POINTER(c_int64)]),
+    ("bst_layer_norm_backward", c_int32, [POINTER(CNormDesc)] + [c_void_p] * 9 + [c_int64, c_void_p]),
+    ("bst_causal_conv_forward", c_int32, [POINTER(CConvDesc)] + [c_void_p] * 8),
+    ("bst_causal_conv_workspace", c_int32, [POINTER(CConvDesc), POINTER(c_int64)]),
+    ("bst_causal_conv_backward", c_int32, [POINTER(CConvDesc)] + [c_void_p] * 12 + [c_int64, c_void_p]),
+    ("bst_causal_conv_step", c_int32,
+     [POINTER(CConvDesc), c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    ("bst_scan_workspace", c_int32, [POINTER(CScanDesc), c_int32, POINTER(c_int64)]),
+    ("bst_scan_forward", c_int32, [POINTER(CScanDesc)] + [c_void_p] * 14 + [c_int64, c_void_p]),
+    ("bst_scan_backward", c_int32, [POINTER(CScanDesc)] + [c_void_p] * 23 + [c_int64, c_void_p]),
+    ("bst_scan_step", c_int32,
+     [POINTER(CScanDesc)] + [c_void_p] * 9 + [c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
 ]
 
 _lib = None

@@ -1,0 +1,414 @@
+// bst_norm.cu — layer norm, forward and backward (bst_layer_norm_*).
+//
+// Forward, per row of D entries:  mean = sum x / D,  var = sum (x - mean)^2 / D,
+//   rstd = 1 / sqrt(var + eps),  y = (x - mean) rstd w + b.
+// Backward, with xh = (x - mean) rstd and g = w dy:
+//   dx = rstd (g - sum g / D - xh sum(g xh) / D),   dw = sum_rows dy xh,   db = sum_rows dy.
+//
+// Both move every element once and do a dozen operations on it, so HBM bounds them: a row is held in
+// registers from its only read to its write (the variance is a second sweep over the registers, which
+// costs no traffic and does not cancel as E[x^2] - mean^2 would).  The rows of a block's turn are
+// `slots`, TPR threads each; a block walks over the rows, so that w and the sums for dw and db stay in
+// its threads' registers for the whole pass and leave it once, as one partial row per slot.  A second
+// launch adds the partial rows up in a fixed order.
+#include <algorithm>
+
+#include "bst_layer.cuh"
+
+namespace bst {
+
+constexpr int kNormItems = 16;        // elements of a row per thread
+constexpr int kNormMaxThreads = 1024; // longer rows than 1024 * 16 go through the kernels that re-read
+
+struct NormArgs {
+  const void *x, *w, *b, *dy;
+  void *y, *dx;
+  float *mean, *rstd;             // forward: outputs (may be null)
+  const float *mean_in, *rstd_in; // backward
+  float* part;                    // [slots][2][dim] partial sums of dw, db
+  int64_t rows, xs, ys, dys, dxs;
+  int dim, wide, vec, params;     // wide: parameters are fp32; params: dw or db asked for
+  float eps, inv_dim;
+};
+
+template <typename T>
+__device__ __forceinline__ float param_at(const void* p, int wide, int i) {
+  return wide ? static_cast<const float*>(p)[i] : to_f(static_cast<const T*>(p)[i]);
+}
+
+// Sum of v over the TPR threads of a row's slot, known to all of them.  `buf`: TPR / 32 floats of the slot.
+template <int TPR>
+__device__ __forceinline__ float2 row_sum2(float2 v, float2* buf) {
+  v.x = warp_sum(v.x);
+  v.y = warp_sum(v.y);
+  if constexpr (TPR > 32) {
+    const int t = threadIdx.x % TPR;
+    __syncthreads();  // the previous sum has been read
+    if (t % 32 == 0) buf[t / 32] = v;
+    __syncthreads();
+    v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) {
+      v.x += buf[i].x;
+      v.y += buf[i].y;
+    }
+  }
+  return v;
+}
+
+// First column of chunk k of thread t of a row.
+template <int TPR, int V>
+__device__ __forceinline__ int column(int t, int k) { return (k * TPR + t) * V; }
+
+template <typename T, int TPR, int V>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_forward_kernel(const NormArgs a) {
+  constexpr int NT = TPR < 256 ? 256 : TPR, SLOTS = NT / TPR, NC = kNormItems / V;
+  __shared__ float2 buf[SLOTS][TPR / 32];
+  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  // Every slot of the block makes the same number of turns: the sums hold barriers.
+  for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += int64_t(gridDim.x) * SLOTS) {
+    const int64_t row = row0 + slot;
+    const bool live = row < a.rows;
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    Chunk<T, V> c[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int i = column<TPR, V>(t, k);
+      c[k] = load_chunk<T, V>(x + i, live ? a.dim - i : 0, a.vec);
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += to_f(c[k].v[j]);
+    const float mean = row_sum2<TPR>(make_float2(s, 0.f), buf[slot]).x * a.inv_dim;
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (column<TPR, V>(t, k) + j < a.dim) {
+          const float d = to_f(c[k].v[j]) - mean;
+          q = fmaf(d, d, q);
+        }
+    const float var = row_sum2<TPR>(make_float2(q, 0.f), buf[slot]).x * a.inv_dim;
+    const float rstd = 1.f / sqrtf(var + a.eps);
+    if (!live) continue;
+    if (t == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+    T* y = static_cast<T*>(a.y) + row * a.ys;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int i = column<TPR, V>(t, k);
+      if (i < a.dim) {
+        Chunk<T, V> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (i + j < a.dim) {
+            const float w = a.w ? param_at<T>(a.w, a.wide, i + j) : 1.f;
+            const float b = a.b ? param_at<T>(a.b, a.wide, i + j) : 0.f;
+            o.v[j] = from_f<T>(fmaf((to_f(c[k].v[j]) - mean) * rstd, w, b));
+          }
+        store_chunk<T, V>(y + i, o, a.dim - i, a.vec);
+      }
+    }
+  }
+}
+
+template <typename T, int TPR, int V>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(const NormArgs a) {
+  constexpr int NT = TPR < 256 ? 256 : TPR, SLOTS = NT / TPR, NC = kNormItems / V;
+  __shared__ float2 buf[SLOTS][TPR / 32];
+  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  float w[kNormItems], dw[kNormItems], db[kNormItems];
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = column<TPR, V>(t, k) + j;
+      w[k * V + j] = a.w && i < a.dim ? param_at<T>(a.w, a.wide, i) : 1.f;
+      dw[k * V + j] = db[k * V + j] = 0.f;
+    }
+  for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += int64_t(gridDim.x) * SLOTS) {
+    const int64_t row = row0 + slot;
+    const bool live = row < a.rows;
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dys;
+    Chunk<T, V> cx[NC], cd[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int i = column<TPR, V>(t, k);
+      cx[k] = load_chunk<T, V>(x + i, live ? a.dim - i : 0, a.vec);
+      cd[k] = load_chunk<T, V>(dy + i, live ? a.dim - i : 0, a.vec);
+    }
+    const float mean = live ? a.mean_in[row] : 0.f, rstd = live ? a.rstd_in[row] : 0.f;
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        // Columns beyond dim hold dy = 0, so that only their xh has to be kept out of nothing.
+        const float d = to_f(cd[k].v[j]);
+        const float xh = (to_f(cx[k].v[j]) - mean) * rstd;
+        const float g = d * w[k * V + j];
+        s.x += g;
+        s.y = fmaf(g, xh, s.y);
+        dw[k * V + j] = fmaf(d, xh, dw[k * V + j]);
+        db[k * V + j] += d;
+      }
+    s = row_sum2<TPR>(s, buf[slot]);
+    const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
+    if (!live) continue;
+    T* dx = static_cast<T*>(a.dx) + row * a.dxs;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int i = column<TPR, V>(t, k);
+      Chunk<T, V> o;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float xh = (to_f(cx[k].v[j]) - mean) * rstd;
+        o.v[j] = from_f<T>(rstd * (to_f(cd[k].v[j]) * w[k * V + j] - m1 - xh * m2));
+      }
+      store_chunk<T, V>(dx + i, o, a.dim - i, a.vec);
+    }
+  }
+  if (!a.params) return;
+  float* p = a.part + (int64_t(blockIdx.x) * SLOTS + slot) * 2 * a.dim;
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = column<TPR, V>(t, k) + j;
+      if (i < a.dim) {
+        p[i] = dw[k * V + j];
+        p[a.dim + i] = db[k * V + j];
+      }
+    }
+}
+
+// ---- rows too long for a block's registers: the row is read again for each sum ------------
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_forward_long_kernel(const NormArgs a) {
+  __shared__ float2 buf[32];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    T* y = static_cast<T*>(a.y) + row * a.ys;
+    float s = 0.f, q = 0.f;
+    for (int i = threadIdx.x; i < a.dim; i += 1024) s += to_f(x[i]);
+    const float mean = row_sum2<1024>(make_float2(s, 0.f), buf).x * a.inv_dim;
+    for (int i = threadIdx.x; i < a.dim; i += 1024) {
+      const float d = to_f(x[i]) - mean;
+      q = fmaf(d, d, q);
+    }
+    const float rstd = 1.f / sqrtf(row_sum2<1024>(make_float2(q, 0.f), buf).x * a.inv_dim + a.eps);
+    if (threadIdx.x == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+    for (int i = threadIdx.x; i < a.dim; i += 1024) {
+      const float w = a.w ? param_at<T>(a.w, a.wide, i) : 1.f, b = a.b ? param_at<T>(a.b, a.wide, i) : 0.f;
+      y[i] = from_f<T>(fmaf((to_f(x[i]) - mean) * rstd, w, b));
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_backward_long_kernel(const NormArgs a) {
+  __shared__ float2 buf[32];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dys;
+    T* dx = static_cast<T*>(a.dx) + row * a.dxs;
+    const float mean = a.mean_in[row], rstd = a.rstd_in[row];
+    float2 s = make_float2(0.f, 0.f);
+    for (int i = threadIdx.x; i < a.dim; i += 1024) {
+      const float g = to_f(dy[i]) * (a.w ? param_at<T>(a.w, a.wide, i) : 1.f);
+      s.x += g;
+      s.y = fmaf(g, (to_f(x[i]) - mean) * rstd, s.y);
+    }
+    s = row_sum2<1024>(s, buf);
+    const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
+    for (int i = threadIdx.x; i < a.dim; i += 1024) {
+      const float g = to_f(dy[i]) * (a.w ? param_at<T>(a.w, a.wide, i) : 1.f);
+      dx[i] = from_f<T>(rstd * (g - m1 - (to_f(x[i]) - mean) * rstd * m2));
+    }
+  }
+}
+
+// Partial rows of dw and db for those: blockIdx.y takes every gridDim.y-th row.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_params_long_kernel(const NormArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.dim) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float d = to_f(static_cast<const T*>(a.dy)[row * a.dys + i]);
+    dw = fmaf(d, (to_f(static_cast<const T*>(a.x)[row * a.xs + i]) - a.mean_in[row]) * a.rstd_in[row], dw);
+    db += d;
+  }
+  float* p = a.part + int64_t(blockIdx.y) * 2 * a.dim;
+  p[i] = dw;
+  p[a.dim + i] = db;
+}
+
+// dw, db = sums of `slots` partial rows of 2 * dim values.  32 columns a block, 32 threads a column.
+template <typename P>
+__global__ void __launch_bounds__(1024) norm_params_kernel(const float* part, int64_t slots, int dim, P* dw, P* db) {
+  __shared__ float sums[32][33];
+  const int c = threadIdx.x % 32, r = threadIdx.x / 32;
+  const int64_t i = int64_t(blockIdx.x) * 32 + c, n = 2 * int64_t(dim);
+  float s = 0.f;
+  if (i < n)
+    for (int64_t k = r; k < slots; k += 32) s += part[k * n + i];
+  sums[r][c] = s;
+  __syncthreads();
+  s = warp_sum(sums[c][r]);  // warp r now adds up column r of the block
+  const int64_t o = int64_t(blockIdx.x) * 32 + r;
+  if (c == 0 && o < n) {
+    if (o < dim) {
+      if (dw) dw[o] = from_f<P>(s);
+    } else if (db) {
+      db[o - dim] = from_f<P>(s);
+    }
+  }
+}
+
+// Threads per row: the fewest of 32, 128, .. 1024 that hold it (0: none does).
+static int norm_threads(int64_t dim) {
+  for (int t : {32, 128, 256, 512, kNormMaxThreads})
+    if (dim <= int64_t(t) * kNormItems) return t;
+  return 0;
+}
+constexpr int kNormBlocksPerSm = 2;  // of the backward pass: each of its slots leaves a partial row
+
+static int64_t norm_backward_blocks(int64_t rows, int tpr) {
+  const int slots = tpr < 256 ? 256 / tpr : 1;
+  return std::max<int64_t>(1, std::min<int64_t>((rows + slots - 1) / slots, int64_t(sm_count()) * kNormBlocksPerSm));
+}
+static int64_t norm_slots(const bst_norm_desc* d) {
+  const int tpr = norm_threads(d->dim);
+  if (tpr == 0) return std::min<int64_t>(std::max<int64_t>(d->rows, 1), 64);
+  return norm_backward_blocks(d->rows, tpr) * (tpr < 256 ? 256 / tpr : 1);
+}
+
+static int norm_check(const bst_norm_desc* d) {
+  if (!d) return fail(BST_ERR_INVALID, "null description");
+  if (!layer_dtype(d->dtype)) return fail(BST_ERR_UNSUPPORTED, "layer norm runs in float32, bfloat16 or float16");
+  if (d->param_dtype != d->dtype && d->param_dtype != BST_F32)
+    return fail(BST_ERR_UNSUPPORTED, "layer norm parameters must have the input's type or float32");
+  if (d->rows < 0 || d->dim < 0) return fail(BST_ERR_INVALID, "negative extent");
+  if (d->dim > (int64_t(1) << 30)) return fail(BST_ERR_UNSUPPORTED, "rows of more than 2^30 entries");
+  if (!(d->eps >= 0)) return fail(BST_ERR_INVALID, "eps must be non-negative");
+  return BST_OK;
+}
+
+template <typename T, bool BWD>
+static int norm_launch(const NormArgs& a, int tpr, unsigned blocks, cudaStream_t st) {
+  constexpr int VW = 16 / int(sizeof(T));
+  auto go = [&](auto tprc, auto vc) {
+    constexpr int TPR = decltype(tprc)::value, V = decltype(vc)::value;
+    constexpr int NT = TPR < 256 ? 256 : TPR;
+    if constexpr (BWD) norm_backward_kernel<T, TPR, V><<<blocks, NT, 0, st>>>(a);
+    else norm_forward_kernel<T, TPR, V><<<blocks, NT, 0, st>>>(a);
+    return launched(BWD ? "norm_backward_kernel launch" : "norm_forward_kernel launch");
+  };
+  auto pick = [&](auto tprc) {
+    return a.vec ? go(tprc, std::integral_constant<int, VW>{}) : go(tprc, std::integral_constant<int, 1>{});
+  };
+  switch (tpr) {
+    case 32: return pick(std::integral_constant<int, 32>{});
+    case 128: return pick(std::integral_constant<int, 128>{});
+    case 256: return pick(std::integral_constant<int, 256>{});
+    case 512: return pick(std::integral_constant<int, 512>{});
+    default: return pick(std::integral_constant<int, 1024>{});
+  }
+}
+
+}  // namespace bst
+
+using namespace bst;
+
+extern "C" {
+
+int bst_layer_norm_forward(const bst_norm_desc* d, const void* x, const void* weight, const void* bias, void* y,
+                           float* mean, float* rstd, void* stream) {
+  clear_error();
+  if (int rc = norm_check(d)) return rc;
+  if (d->rows == 0 || d->dim == 0) return BST_OK;
+  if (!x || !y) return fail(BST_ERR_INVALID, "null device pointer");
+  const int64_t es = layer_elem_size(d->dtype), per = 16 / es;
+  NormArgs a{};
+  a.x = x, a.w = weight, a.b = bias, a.y = y, a.mean = mean, a.rstd = rstd;
+  a.rows = d->rows, a.xs = d->x_row, a.ys = d->y_row, a.dim = int(d->dim);
+  a.wide = d->param_dtype == BST_F32 && d->dtype != BST_F32;
+  a.vec = aligned16(x) && aligned16(y) && d->dim % per == 0 && d->x_row % per == 0 && d->y_row % per == 0;
+  a.eps = float(d->eps), a.inv_dim = 1.f / float(d->dim);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int tpr = norm_threads(d->dim);
+  const int slots = tpr && tpr < 256 ? 256 / tpr : 1;
+  const unsigned blocks = unsigned(std::min<int64_t>((d->rows + slots - 1) / slots, INT_MAX));
+  return with_type(d->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (tpr) return norm_launch<T, false>(a, tpr, blocks, st);
+    norm_forward_long_kernel<T><<<blocks, 1024, 0, st>>>(a);
+    return launched("norm_forward_long_kernel launch");
+  });
+}
+
+int bst_layer_norm_workspace(const bst_norm_desc* d, int64_t* bytes) {
+  clear_error();
+  if (int rc = norm_check(d)) return rc;
+  if (!bytes) return fail(BST_ERR_INVALID, "null output");
+  *bytes = d->rows == 0 || d->dim == 0 ? 0 : norm_slots(d) * 2 * d->dim * 4;
+  return BST_OK;
+}
+
+int bst_layer_norm_backward(const bst_norm_desc* d, const void* x, const void* weight, const void* dy,
+                            const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+  int64_t need = 0;
+  if (int rc = bst_layer_norm_workspace(d, &need)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t es = layer_elem_size(d->dtype), per = 16 / es, ps = layer_elem_size(d->param_dtype);
+  if (d->dim == 0) return BST_OK;
+  if (d->rows == 0) {
+    if (dweight) BST_CUDA(cudaMemsetAsync(dweight, 0, size_t(d->dim * ps), st));
+    if (dbias) BST_CUDA(cudaMemsetAsync(dbias, 0, size_t(d->dim * ps), st));
+    return BST_OK;
+  }
+  if (!x || !dy || !dx || !mean || !rstd) return fail(BST_ERR_INVALID, "null device pointer");
+  const bool params = dweight || dbias;
+  if (params && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(BST_ERR_INVALID, "the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
+  NormArgs a{};
+  a.x = x, a.w = weight, a.dy = dy, a.dx = dx, a.mean_in = mean, a.rstd_in = rstd;
+  a.part = static_cast<float*>(workspace);
+  a.rows = d->rows, a.xs = d->x_row, a.dys = d->dy_row, a.dxs = d->dx_row, a.dim = int(d->dim);
+  a.wide = d->param_dtype == BST_F32 && d->dtype != BST_F32;
+  a.vec = aligned16(x) && aligned16(dy) && aligned16(dx) && d->dim % per == 0 && d->x_row % per == 0 &&
+          d->dy_row % per == 0 && d->dx_row % per == 0;
+  a.params = params;
+  a.inv_dim = 1.f / float(d->dim);
+  const int tpr = norm_threads(d->dim);
+  int rc = with_type(d->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (tpr) return norm_launch<T, true>(a, tpr, unsigned(norm_backward_blocks(d->rows, tpr)), st);
+    norm_backward_long_kernel<T><<<unsigned(std::min<int64_t>(d->rows, INT_MAX)), 1024, 0, st>>>(a);
+    if (int e = launched("norm_backward_long_kernel launch")) return e;
+    if (!params) return int(BST_OK);
+    norm_params_long_kernel<T><<<dim3(unsigned((d->dim + 255) / 256), unsigned(norm_slots(d))), 256, 0, st>>>(a);
+    return launched("norm_params_long_kernel launch");
+  });
+  if (rc || !params) return rc;
+  const unsigned blocks = unsigned((2 * d->dim + 31) / 32);
+  return with_type(d->param_dtype, [&](auto t) {
+    using P = decltype(t);
+    norm_params_kernel<P><<<blocks, 1024, 0, st>>>(a.part, norm_slots(d), a.dim, static_cast<P*>(dweight),
+                                                   static_cast<P*>(dbias));
+    return launched("norm_params_kernel launch");
+  });
+}
+
+}  // extern "C"

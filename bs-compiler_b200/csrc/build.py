@@ -31,7 +31,8 @@ NVFLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-fmad=false", "--expt-relax
                   "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", f"-I{INCLUDE}"]
 NVFLAGS += os.environ.get("BST_NVCC_EXTRA", "").split()  # e.g. tile-size macros for tuning builds
 
-KERNEL_UNITS = ["bst_core.cu", "bst_f32.cu", "bst_f64.cu", "bst_interceptor.cu", "bst_halo.cu", "bst_noalloc.cu"]
+KERNEL_UNITS = ["bst_core.cu", "bst_f32.cu", "bst_f64.cu", "bst_interceptor.cu", "bst_halo.cu", "bst_noalloc.cu",
+                "bst_norm.cu", "bst_conv.cu", "bst_scan.cu", "bst_scan_backward.cu", "bst_scan_step.cu"]
 HEADERS = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "basalto_b200.h"]
 
 LIB = PKG / "libbasalto_b200.so"

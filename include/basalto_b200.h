@@ -1,5 +1,5 @@
 /*
- * basalto_b200.h — C ABI of the B200-native Basalto stencil hot path.
+ * basalto_b200.h — C ABI of the B200-native Basalto stencil hot path and layer operators.
  *
  * Plain C: pointers, sizes and status codes only; no torch or C++ types cross this
  * boundary.  Device pointers are raw CUDA device addresses in the caller's current
@@ -44,7 +44,8 @@ typedef enum bst_status {
 } bst_status;
 
 /* ---- element types ------------------------------------------------------------- */
-typedef enum bst_dtype { BST_F32 = 0, BST_F64 = 1 } bst_dtype;
+/* Stencils run in F32 and F64, the layer operators below in F32, BF16 and F16. */
+typedef enum bst_dtype { BST_F32 = 0, BST_F64 = 1, BST_BF16 = 2, BST_F16 = 3 } bst_dtype;
 
 /* ---- stencil program ("grouped linear stencil") ---------------------------------
  * out(p) = fold+( term_0, term_1, ..., term_{nterms-1} )       left fold: ((t0+t1)+t2)+...
@@ -333,6 +334,115 @@ BST_API int bst_comm_profile_end(bst_comm* c, double out[6]);
  * picks the plan.  One band when out[0] == tiles. */
 BST_API int bst_march_item_plan(int64_t tiles, int64_t planes, int32_t rb, int32_t overhead, int64_t resident,
                                 int64_t out[5]);
+
+/* ---- layer operators --------------------------------------------------------------
+ * The operators of a state space layer that the torch.compile backend can run next to
+ * stencils: layer norm, the short causal depthwise convolution (a one-sided 1-D stencil with
+ * weights of its own for every channel) and the selective scan (a linear recurrence stepped
+ * along the same axis).  The reference has none of them: its backend leaves such graphs to
+ * eager execution (python/basalto/compiler.py:44-75).
+ *
+ * Element types: `dtype` (F32, BF16 or F16) for the activations; arithmetic, sums and
+ * states are fp32, and each result is rounded once.  Strides are in elements; the innermost
+ * axis of every tensor is contiguous unless stated otherwise.  Optional pointers are NULL
+ * when absent.  Every call queues its kernels on `stream` of the current device, allocates
+ * nothing and can be captured into a CUDA graph; workspaces are the caller's, must be aligned
+ * to 16 bytes, and belong to one call at a time (two calls that may overlap need two).
+ * Results do not depend on the order in which blocks run (no atomics).
+ * Empty problems (no rows, no batch, no channels) return BST_OK; a reduction over nothing
+ * (gradients of parameters) is then zero. */
+
+/* Layer norm over the last axis of [rows, dim]:
+ *   y = (x - mean) * rstd * weight + bias,   rstd = 1 / sqrt(var + eps)  (biased variance)
+ * weight and bias (dim entries of param_dtype, which is dtype or F32) are optional. */
+typedef struct bst_norm_desc {
+  int32_t dtype, param_dtype;
+  int64_t rows, dim;
+  int64_t x_row, y_row, dy_row, dx_row; /* elements from one row to the next */
+  double eps;
+} bst_norm_desc;
+/* mean and rstd (fp32, one per row) are optional outputs; the backward pass reads them. */
+BST_API int bst_layer_norm_forward(const bst_norm_desc* d, const void* x, const void* weight, const void* bias,
+                                   void* y, float* mean, float* rstd, void* stream);
+/* Bytes of workspace that bst_layer_norm_backward needs for this description. */
+BST_API int bst_layer_norm_workspace(const bst_norm_desc* d, int64_t* bytes);
+/* dx, and where asked for (non-NULL) dweight and dbias, in param_dtype. */
+BST_API int bst_layer_norm_backward(const bst_norm_desc* d, const void* x, const void* weight, const void* dy,
+                                    const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Causal depthwise convolution of x [batch, length, channels]:
+ *   p[t, c] = bias[c] + sum_k weight[c, k] x[t - width + 1 + k, c],   y = p, or p sigmoid(p) (silu)
+ * Inputs before the first are initial's [batch, width - 1, channels] (NULL: zeros).  lengths
+ * (int32, one per sequence, clamped to [0, length]; NULL: all `length`): y is zero from
+ * lengths[b] on, x there is not read, and final (optional, [batch, width - 1, channels]) holds
+ * the last width - 1 inputs before lengths[b].  weight [channels, width] is contiguous; initial
+ * and final are contiguous.  Either the channel axis (lines = 0) or the sequence axis (lines = 1)
+ * of x, y, dy and dx is contiguous: `*_step` is the stride of the other one.  width 1..8. */
+typedef struct bst_conv_desc {
+  int32_t dtype, param_dtype; /* param_dtype (weight, bias and their gradients): dtype or F32 */
+  int32_t width, silu, lines;
+  int64_t batch, length, channels;
+  int64_t x_batch, x_step, y_batch, y_step, dy_batch, dy_step, dx_batch, dx_step;
+} bst_conv_desc;
+BST_API int bst_causal_conv_forward(const bst_conv_desc* d, const void* x, const void* weight, const void* bias,
+                                    const void* initial, const int32_t* lengths, void* y, void* final_state,
+                                    void* stream);
+BST_API int bst_causal_conv_workspace(const bst_conv_desc* d, int64_t* bytes);
+/* dx, dweight, and where asked for dbias and dinitial; dfinal (optional) is the gradient of
+ * final's entries.  dx is zero from lengths[b] on. */
+BST_API int bst_causal_conv_backward(const bst_conv_desc* d, const void* x, const void* weight, const void* bias,
+                                     const void* initial, const int32_t* lengths, const void* dy,
+                                     const void* dfinal, void* dx, void* dweight, void* dbias, void* dinitial,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+/* One position: x, y [batch, channels] (x_batch, y_batch apart), state [batch, width - 1,
+ * channels] (oldest first; state_batch apart, rows contiguous).  out_state receives the state
+ * with x appended and the oldest input dropped; it may be `state` itself (in place), and may not
+ * overlap it otherwise.  length, lines and the other strides of the description are not used. */
+BST_API int bst_causal_conv_step(const bst_conv_desc* d, const void* x, const void* state, int64_t state_batch,
+                                 const void* weight, const void* bias, void* y, void* out_state,
+                                 int64_t out_state_batch, void* stream);
+
+/* Selective scan: per batch entry and channel c (of group g = c / (channels / groups)), with a
+ * state h of `states` fp32 entries,
+ *   d_t = softplus(delta_t + delta_bias)  (or delta_t + delta_bias, softplus = 0)
+ *   h_t[n] = exp(d_t A[c, n]) h_{t-1}[n] + d_t u_t B_t[g, n]
+ *   y_t = (sum_n C_t[g, n] h_t[n] + D[c] u_t) z_t sigmoid(z_t)      (no z: no gate)
+ * u, delta, z, y: [batch, length, channels]; B, C: [batch, length, groups, states]; A [channels,
+ * states], D, delta_bias [channels], initial and final [batch, channels, states]: fp32,
+ * contiguous.  delta_bias, D, z, initial (zeros) and lengths (as above) are optional; final is
+ * the state after lengths[b] steps.  states 1..64; groups divides channels.
+ * A workspace of bst_scan_workspace(.., BST_SCAN_FORWARD) bytes may be needed.  `saved` (NULL,
+ * or BST_SCAN_SAVED bytes) receives the states that the backward pass starts from. */
+typedef struct bst_scan_desc {
+  int32_t dtype, softplus;
+  int64_t batch, length, channels, states, groups;
+  int64_t u_batch, u_step, delta_batch, delta_step, z_batch, z_step, y_batch, y_step, dy_batch, dy_step;
+  int64_t B_batch, B_step, B_group, C_batch, C_step, C_group;
+} bst_scan_desc;
+enum { BST_SCAN_FORWARD = 0, BST_SCAN_BACKWARD = 1, BST_SCAN_SAVED = 2 };
+BST_API int bst_scan_workspace(const bst_scan_desc* d, int32_t what, int64_t* bytes);
+BST_API int bst_scan_forward(const bst_scan_desc* d, const void* u, const void* delta, const float* A, const void* B,
+                             const void* C, const float* D, const void* z, const float* delta_bias,
+                             const float* initial, const int32_t* lengths, void* y, float* final_state, void* saved,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients, contiguous: du, ddelta, dz [batch, length, channels] and dB, dC [batch, length,
+ * groups, states] in dtype; dA, dD, ddelta_bias, dinitial in fp32.  dz, dD, ddelta_bias and
+ * dinitial are optional; dfinal (optional) is the gradient of final.  Positions from
+ * lengths[b] on get zeros. */
+BST_API int bst_scan_backward(const bst_scan_desc* d, const void* u, const void* delta, const float* A, const void* B,
+                              const void* C, const float* D, const void* z, const float* delta_bias,
+                              const int32_t* lengths, const void* dy, const float* dfinal, const void* saved,
+                              void* du, void* ddelta, float* dA, void* dB, void* dC, float* dD, void* dz,
+                              float* ddelta_bias, float* dinitial, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+/* One position: the description's *_batch strides (B_group, C_group) with length 1; state and
+ * out_state [batch, channels, states] fp32, `*_batch` and `*_channel` apart.  out_state may be
+ * `state` itself (in place), and may not overlap it otherwise. */
+BST_API int bst_scan_step(const bst_scan_desc* d, const void* u, const void* delta, const float* A, const void* B,
+                          const void* C, const float* D, const void* z, const float* delta_bias, const float* state,
+                          int64_t state_batch, int64_t state_channel, void* y, float* out_state,
+                          int64_t out_batch, int64_t out_channel, void* stream);
 
 #ifdef __cplusplus
 }
