@@ -22,6 +22,12 @@ attention / softmax branches, compiler.py:10-75) are returned unchanged and run 
 which is exactly what the reference does for them; set BASALTO_FALLBACK_EAGER=0 to make
 that an error instead.  Stencil graphs called with CPU tensors raise: the kernels run on
 CUDA devices only.
+
+BASALTO_MODEL_OPS=1 also sends the layer norms and causal depthwise convolutions of such a graph
+to the layer kernels (fx_layers.route), with their gradients; the rest of it runs eagerly.  It is
+off by default, because their results differ from eager torch's by rounding.  Graphs in which the
+user's code calls basalto.layer_norm, causal_conv or selective_scan run those on the kernels in any
+case.  With BASALTO_FALLBACK_EAGER=0 a graph that has such a node is no error.
 """
 from __future__ import annotations
 
@@ -34,6 +40,7 @@ import torch.fx
 
 from . import _rust
 from .fx_extract import Unsupported, extract
+from .fx_layers import has_layer_ops, route
 
 log = logging.getLogger("basalto")
 
@@ -42,6 +49,10 @@ _tls = threading.local()
 
 def _fp_contract() -> bool:
     return os.environ.get("BASALTO_FP_CONTRACT", "0") == "1"
+
+
+def _model_ops() -> bool:
+    return os.environ.get("BASALTO_MODEL_OPS", "0") == "1"
 
 
 def _extract(gm, args):
@@ -112,6 +123,10 @@ def basalto_backend(gm: torch.fx.GraphModule, example_inputs):
     try:
         prog, tin = _extract(gm, list(example_inputs))
     except Unsupported as e:
+        if _model_ops() and route(gm):
+            return gm
+        if has_layer_ops(gm):
+            return gm
         if os.environ.get("BASALTO_FALLBACK_EAGER", "1") == "0":
             raise RuntimeError(f"basalto: graph is not a supported stencil ({e})") from e
         log.info("basalto: running graph eagerly (%s)", e)

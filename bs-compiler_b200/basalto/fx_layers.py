@@ -1,0 +1,157 @@
+"""Layer operators in the graphs that Dynamo hands the backend.
+
+`route(gm)` looks for nodes that the layer kernels can run on CUDA tensors in float32, bfloat16 or float16:
+
+* F.layer_norm over the last axis;
+* F.conv1d that is depthwise and causal: stride and dilation 1, groups = channels, 1 to 8 taps, and either padded
+  by taps - 1 on both sides and cut back to the sequence ([..., :length]), or over an F.pad(x, (taps - 1, 0)) of
+  zeros; a silu of the result that nothing else reads goes into the same kernel.
+
+It replaces them and returns how many it replaced.  Their gradients are the kernels' own.  Shapes and types are
+those of Dynamo's example values; nodes without them, or with symbolic sizes, are left alone.
+`has_layer_ops(gm)`: whether the user's code itself called one of the custom operators torch.ops.basalto.*.
+"""
+from __future__ import annotations
+
+import operator
+
+import torch
+import torch.nn.functional as F
+
+from . import layers
+
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_SILU = {F.silu, torch.ops.aten.silu.default}
+_PAD = {F.pad, getattr(torch._C._nn, "pad", F.pad)}
+_CONV = {F.conv1d, torch.conv1d}
+
+
+def _value(n):
+    """The example tensor of a node, if its sizes are plain numbers."""
+    v = n.meta.get("example_value") if isinstance(n, torch.fx.Node) else None
+    if not isinstance(v, torch.Tensor) or any(not isinstance(s, int) for s in (*v.shape, *v.stride())):
+        return None
+    return v
+
+
+def _usable(*values):
+    return all(v is not None and v.is_cuda and v.dtype in _TYPES and v.device == values[0].device for v in values)
+
+
+def _arg(n, i, name, default=None):
+    return n.args[i] if len(n.args) > i else n.kwargs.get(name, default)
+
+
+def _param_ok(p, x):
+    """A parameter node that the kernels take with x (None: absent)."""
+    if p is None:
+        return True
+    v = _value(p)
+    return _usable(x, v) and v.dtype in (x.dtype, torch.float32)
+
+
+def _same_type(*ps):
+    return len({_value(p).dtype for p in ps if p is not None}) <= 1
+
+
+def _layer_norm(n):
+    x = _value(_arg(n, 0, "input"))
+    shape = _arg(n, 1, "normalized_shape")
+    w, b, eps = _arg(n, 2, "weight"), _arg(n, 3, "bias"), _arg(n, 4, "eps", 1e-5)
+    if x is None or not _usable(x) or not isinstance(eps, (int, float)):
+        return None
+    shape = (shape,) if isinstance(shape, int) else tuple(shape)
+    if x.dim() < 1 or shape != (x.shape[-1],) or not (_param_ok(w, x) and _param_ok(b, x) and _same_type(w, b)):
+        return None
+    return layers.layer_norm, (_arg(n, 0, "input"), w, b, float(eps))
+
+
+def _one(v, want):
+    return v == want or (isinstance(v, (tuple, list)) and len(v) == 1 and v[0] == want)
+
+
+def conv_channels_first(x, weight, bias, activation):
+    """causal_conv of x [batch, channels, length] with conv1d's weight [channels, 1, taps]."""
+    return layers.causal_conv(x.transpose(1, 2), weight.squeeze(1), bias, activation).transpose(1, 2)
+
+
+def _causal_conv(n):
+    """(last node of the pattern, x, weight, bias) of a causal depthwise convolution at conv1d node n."""
+    x, w, b = _arg(n, 0, "input"), _arg(n, 1, "weight"), _arg(n, 2, "bias")
+    stride, pad = _arg(n, 3, "stride", 1), _arg(n, 4, "padding", 0)
+    dilation, groups = _arg(n, 5, "dilation", 1), _arg(n, 6, "groups", 1)
+    xv, wv = _value(x), _value(w)
+    if xv is None or wv is None or not _usable(xv, wv) or xv.dim() != 3 or wv.dim() != 3:
+        return None
+    c, taps = xv.shape[1], wv.shape[2]
+    if groups != c or tuple(wv.shape) != (c, 1, taps) or not 1 <= taps <= 8 or not (_one(stride, 1) and
+                                                                                    _one(dilation, 1)):
+        return None
+    if not (_param_ok(w, xv) and _param_ok(b, xv) and _same_type(w, b)):
+        return None
+    if _one(pad, 0) and isinstance(x, torch.fx.Node) and x.target in _PAD and x.op == "call_function":
+        spec = tuple(_arg(x, 1, "pad"))
+        src = _value(_arg(x, 0, "input"))
+        if (src is not None and spec == (taps - 1, 0) and _arg(x, 2, "mode", "constant") == "constant"
+                and _arg(x, 3, "value") in (None, 0, 0.0)):
+            return n, _arg(x, 0, "input"), w, b
+        return None
+    if taps == 1 and _one(pad, 0):
+        return n, x, w, b
+    if not _one(pad, taps - 1) or len(n.users) != 1:
+        return None
+    cut = next(iter(n.users))
+    if cut.op != "call_function" or cut.target is not operator.getitem:
+        return None
+    idx = cut.args[1]
+    lead, last = (idx[:-1], idx[-1]) if isinstance(idx, tuple) else ((), None)
+    whole = all(i is Ellipsis or i == slice(None, None, None) for i in lead)
+    if not whole or (len(idx) != 3 and not (len(idx) == 2 and lead[0] is Ellipsis)):
+        return None
+    length = xv.shape[2]
+    if not isinstance(last, slice) or last.start not in (None, 0) or last.step not in (None, 1):
+        return None
+    if last.stop != length and not (taps > 1 and last.stop == 1 - taps):
+        return None
+    return cut, x, w, b
+
+
+def _replace(gm, node, fn, args):
+    with gm.graph.inserting_before(node):
+        new = gm.graph.call_function(fn, args)
+    new.meta = dict(node.meta)
+    node.replace_all_uses_with(new)
+
+
+def has_layer_ops(gm: torch.fx.GraphModule) -> bool:
+    return any(n.op == "call_function" and getattr(n.target, "namespace", str(n.target).split(".")[0]) == "basalto"
+               for n in gm.graph.nodes)
+
+
+def route(gm: torch.fx.GraphModule) -> int:
+    """Replace what the layer kernels can run, in place; returns how many nodes were replaced."""
+    count = 0
+    for n in list(gm.graph.nodes):
+        if n.op != "call_function":
+            continue
+        if n.target is F.layer_norm:
+            hit = _layer_norm(n)
+            if hit:
+                _replace(gm, n, *hit)
+                count += 1
+        elif n.target in _CONV:
+            hit = _causal_conv(n)
+            if hit:
+                last, x, w, b = hit
+                act = None
+                if len(last.users) == 1:
+                    user = next(iter(last.users))
+                    if user.op == "call_function" and user.target in _SILU and not user.kwargs.get("inplace") and \
+                            len(user.args) == 1:
+                        last, act = user, "silu"
+                _replace(gm, last, conv_channels_first, (x, w, b, act))
+                count += 1
+    if count:
+        gm.graph.eliminate_dead_code()
+        gm.recompile()
+    return count
