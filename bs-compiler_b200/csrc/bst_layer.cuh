@@ -91,9 +91,7 @@ __device__ __forceinline__ float softplus(float x) {
   p = fmaf(p, q, 1.f / 5.f);
   p = fmaf(p, q, 1.f / 3.f);
   p = fmaf(p, q, 1.f);
-  // NaN: fmaxf would drop it, the sum with x - x keeps it (0 for finite x, +inf has t = 0 already).
-  const float r = fmaf(2.f * s, p, fmaxf(x, 0.f));
-  return x == x ? r : x;
+  return fmaf(2.f * s, p, x < 0.f ? 0.f : x);  // a NaN is kept: x < 0 is false for it
 }
 
 // Two fp32 lanes per instruction.
@@ -101,6 +99,31 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// sigmoid and softplus of two values, their fused operations paired.
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
+  const float2 e = ex2_2(mul2(x, both(-kLog2e)));
+  const float2 d = add2(e, both(1.f));
+  return make_float2(rcp(d.x), rcp(d.y));
+}
+__device__ __forceinline__ float2 softplus2(float2 x) {
+  const float2 t = ex2_2(make_float2(-fabsf(x.x) * kLog2e, -fabsf(x.y) * kLog2e));
+  const float2 w = add2(t, both(2.f));
+  const float2 s = mul2(t, make_float2(rcp(w.x), rcp(w.y)));
+  const float2 q = mul2(s, s);
+  float2 p = both(1.f / 13.f);
+  p = fma2(p, q, both(1.f / 11.f));
+  p = fma2(p, q, both(1.f / 9.f));
+  p = fma2(p, q, both(1.f / 7.f));
+  p = fma2(p, q, both(1.f / 5.f));
+  p = fma2(p, q, both(1.f / 3.f));
+  p = fma2(p, q, both(1.f));
+  // max(x, 0) that keeps a NaN: x < 0 is false for it.
+  const float2 m = make_float2(x.x < 0.f ? 0.f : x.x, x.y < 0.f ? 0.f : x.y);
+  return fma2(add2(s, s), p, m);
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -1,5 +1,6 @@
 // bst_scan.cu — selective scan: forward pass (bst_scan_forward) and workspace sizes.
 #include <algorithm>
+#include <cstdlib>
 
 #include "bst_scan.cuh"
 
@@ -8,17 +9,19 @@ namespace bst {
 // One block: CT channels of one sequence, its tiles in order.
 template <typename T, class Sh>
 __global__ void __launch_bounds__(Sh::NT) scan_forward_kernel(const ScanArgs a) {
-  constexpr int S = Sh::S, GS = Sh::GS, PW = Sh::PW, CT = Sh::CT, NP = Sh::NP, NT = Sh::NT;
+  constexpr int S = Sh::S, CH = Sh::CH, GS = Sh::GS, CT = Sh::CT, NP = Sh::NP, NT = Sh::NT;
   using Share = TileShare<T, Sh>;
-  constexpr int V = Share::V, CNT = Share::CNT;
-  constexpr int BC = kScanTile * NP / NT > 0 ? kScanTile * NP / NT : 1;  // elements of B (of C) per thread
-  __shared__ float4 s_step[kScanTile][CT / 2];  // (d, d', d u, d' u') of a channel pair
-  __shared__ float2 s_B[kScanTile][NP], s_C[kScanTile][NP];  // each value twice, as the paired operands want it
-  __shared__ float s_y[kScanTile][CT];
+  using States = StateShare<T, Sh>;
+  constexpr int V = Share::V, CNT = Share::CNT, VB = States::V;
+  __shared__ Step<CH> s_step[kScanTile][CT / CH];
+  __shared__ __align__(16) float s_B[kScanTile][NP], s_C[kScanTile][NP];
+  __shared__ __align__(16) float s_y[kScanTile][CT];
+  __shared__ Chunk<T, V> s_u[2][CNT][NT], s_dl[2][CNT][NT], s_z[2][CNT][NT];
+  __shared__ Chunk<T, VB> s_rawB[2][States::CNT][NT], s_rawC[2][States::CNT][NT];
 
   const ScanWhere at = scan_where(a);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int sg = lane % GS, pair = warp * PW + lane / GS;
+  const int sg = lane % GS, cell = warp * (32 / GS) + lane / GS;
   const int c0 = at.ct * CT, left = a.per_group - c0;  // channels of the group from this tile on
   const int64_t cbase = int64_t(at.g) * a.per_group + c0;
   const int64_t len = scan_length(a, at.b);
@@ -26,22 +29,18 @@ __global__ void __launch_bounds__(Sh::NT) scan_forward_kernel(const ScanArgs a) 
   const int64_t stop = min(first + int64_t(a.seg_tiles) * kScanTile, a.length);  // of this segment
   const int64_t live = min(stop, len);
 
-  const int c_lane = 2 * pair;
-  float2 h[S], a2[S];
+  const int c_lane = CH * cell;
+  Pairs<S> h[CH], a2[CH];
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const int n = sg * S + s;
-    h[s] = a2[s] = make_float2(0.f, 0.f);
-    if (n < a.states) {
-      if (c_lane < left) a2[s].x = a.A[(cbase + c_lane) * a.states + n] * kLog2e;
-      if (c_lane + 1 < left) a2[s].y = a.A[(cbase + c_lane + 1) * a.states + n] * kLog2e;
-      if (a.init) {
-        const float* p = a.init + (at.b * a.channels + cbase + c_lane) * a.states + n;
-        if (c_lane < left) h[s].x = p[0];
-        if (c_lane + 1 < left) h[s].y = p[a.states];
-      }
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int n = sg * S + s;
+      const bool on = n < a.states && c_lane + c < left;
+      const int64_t i = (cbase + c_lane + c) * a.states + n;
+      (s % 2 ? a2[c].v[s / 2].y : a2[c].v[s / 2].x) = on ? a.A[i] * kLog2e : 0.f;
+      (s % 2 ? h[c].v[s / 2].y : h[c].v[s / 2].x) = on && a.init ? a.init[at.b * a.channels * a.states + i] : 0.f;
     }
-  }
   const int col = Share::col();
   float skip[V], bias[V];
 #pragma unroll
@@ -56,68 +55,100 @@ __global__ void __launch_bounds__(Sh::NT) scan_forward_kernel(const ScanArgs a) 
   const T* B = static_cast<const T*>(a.B) + at.b * a.Bb + at.g * a.Bg;
   const T* C = static_cast<const T*>(a.C) + at.b * a.Cb + at.g * a.Cg;
 
-  for (int64_t t0 = first; t0 < live; t0 += kScanTile) {
+  // Two tiles are on their way while a third is worked on.
+  auto fetch = [&](int64_t t0, int slot) {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int64_t t = t0 + Share::row(i);
+      const int n = t < live ? left - col : 0;
+      stage_chunk<T, V>(&s_u[slot][i][threadIdx.x], u + t * a.us, static_cast<const T*>(a.u), n, a.mode_act);
+      stage_chunk<T, V>(&s_dl[slot][i][threadIdx.x], dl + t * a.ds, static_cast<const T*>(a.delta), n, a.mode_act);
+      if (a.z) stage_chunk<T, V>(&s_z[slot][i][threadIdx.x], z + t * a.zs, static_cast<const T*>(a.z), n, a.mode_act);
+    }
+#pragma unroll
+    for (int i = 0; i < States::CNT; ++i) {
+      const int k = States::item(i), n = States::state(k);
+      const int64_t t = t0 + States::row(k);
+      const int m = k < States::ITEMS && t < live ? a.states - n : 0;
+      stage_chunk<T, VB>(&s_rawB[slot][i][threadIdx.x], B + t * a.Bs + n, B, m, a.mode_bc);
+      stage_chunk<T, VB>(&s_rawC[slot][i][threadIdx.x], C + t * a.Cs + n, C, m, a.mode_bc);
+    }
+  };
+  if (first < live) fetch(first, 0);
+  copy_commit();
+  if (first + kScanTile < live) fetch(first + kScanTile, 1);
+  copy_commit();
+  int slot = 0;
+  for (int64_t t0 = first; t0 < live; t0 += kScanTile, slot ^= 1) {
+    copy_wait<1>();
     Chunk<T, V> cu[CNT], cz[CNT];
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
       const int r = Share::row(i);
-      const int64_t t = t0 + r;
-      const int n = t < live ? left - col : 0;
-      cu[i] = load_chunk<T, V>(u + t * a.us, n, a.vec);
-      const Chunk<T, V> cd = load_chunk<T, V>(dl + t * a.ds, n, a.vec);
-      cz[i] = load_chunk<T, V>(z + t * a.zs, a.z ? n : 0, a.vec);
+      const int n = t0 + r < live ? left - col : 0;
+      cu[i] = s_u[slot][i][threadIdx.x];
+      cz[i] = s_z[slot][i][threadIdx.x];
+      const Chunk<T, V> cd = s_dl[slot][i][threadIdx.x];
+      float d[V], du[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = to_f(cd.v[j]) + bias[j];
+      if (a.softplus) by_two<V>(d, softplus, softplus2);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float raw = to_f(cd.v[j]) + bias[j];
-        const float d = j < n ? (a.softplus ? softplus(raw) : raw) : 0.f;
-        float* cell = reinterpret_cast<float*>(&s_step[r][(col + j) / 2]) + (col + j) % 2;
-        cell[0] = d;
-        cell[2] = d * to_f(cu[i].v[j]);
+        d[j] = j < n ? d[j] : 0.f;
+        du[j] = d[j] * to_f(cu[i].v[j]);
       }
+      put_steps<CH, V>(s_step[r], col, d, du);
     }
 #pragma unroll
-    for (int i = 0; i < BC; ++i) {
-      const int e = threadIdx.x + i * NT, r = e / NP, n = e % NP;
-      if (r < kScanTile) {
-        const bool on = t0 + r < live && n < a.states;
-        const float vb = on ? to_f(B[(t0 + r) * a.Bs + n]) : 0.f, vc = on ? to_f(C[(t0 + r) * a.Cs + n]) : 0.f;
-        s_B[r][n] = make_float2(vb, vb);
-        s_C[r][n] = make_float2(vc, vc);
+    for (int i = 0; i < States::CNT; ++i) {
+      const int k = States::item(i);
+      if (k < States::ITEMS) {
+        const Chunk<T, VB> cb = s_rawB[slot][i][threadIdx.x], cc = s_rawC[slot][i][threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < VB; ++j) {
+          s_B[States::row(k)][States::state(k) + j] = to_f(cb.v[j]);
+          s_C[States::row(k)][States::state(k) + j] = to_f(cc.v[j]);
+        }
       }
     }
     if (a.saved) {
       float* k = a.saved + ((at.b * ((a.length + kScanTile - 1) / kScanTile) + t0 / kScanTile) * a.channels + cbase +
                             c_lane) * NP + sg * S;
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if (c_lane < left) k[s] = h[s].x;
-        if (c_lane + 1 < left) k[NP + s] = h[s].y;
-      }
+      for (int c = 0; c < CH; ++c)
+        if (c_lane + c < left) *reinterpret_cast<Pairs<S>*>(k + c * NP) = h[c];
     }
     __syncthreads();
-    constexpr int U = GS >= 2 ? GS / 2 : 1;  // steps whose sums are joined together
-#pragma unroll 1
+    if (t0 + 2 * kScanTile < live) fetch(t0 + 2 * kScanTile, slot);
+    copy_commit();
+    constexpr int U = GS > CH ? GS / CH : 1;  // steps whose sums over the states are joined together
+    constexpr int OUT = U * CH / GS;          // of which each lane ends with so many
+#pragma unroll
     for (int r0 = 0; r0 < kScanTile; r0 += U) {
-      float v[2 * U];
+      float v[U * CH];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const float4 st = s_step[r0 + j][pair];
-        float2 acc = make_float2(0.f, 0.f);
+        const Step<CH> st = s_step[r0 + j][cell];
+        const Pairs<S> Bn = *reinterpret_cast<const Pairs<S>*>(&s_B[r0 + j][sg * S]);
+        const Pairs<S> Cn = *reinterpret_cast<const Pairs<S>*>(&s_C[r0 + j][sg * S]);
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const float2 e = decay(make_float2(st.x, st.y), a2[s]);
-          h[s] = fma2(e, h[s], mul2(make_float2(st.z, st.w), s_B[r0 + j][sg * S + s]));
-          acc = fma2(h[s], s_C[r0 + j][sg * S + s], acc);
+        for (int c = 0; c < CH; ++c) {
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int s = 0; s < S / 2; ++s) {
+            const float2 e = decay(both(st.d[c]), a2[c].v[s]);
+            h[c].v[s] = fma2(e, h[c].v[s], mul2(both(st.du[c]), Bn.v[s]));
+            acc = s == 0 ? mul2(h[c].v[s], Cn.v[s]) : fma2(h[c].v[s], Cn.v[s], acc);
+          }
+          v[j * CH + c] = acc.x + acc.y;
         }
-        v[2 * j] = acc.x;
-        v[2 * j + 1] = acc.y;
       }
-      if constexpr (GS == 1) {
-        s_y[r0][c_lane] = v[0];
-        s_y[r0][c_lane + 1] = v[1];
-      } else {
-        reduce_scatter<2 * U, GS, 1>(v, lane);
-        s_y[r0 + sg / 2][c_lane + sg % 2] = v[0];
+      reduce_scatter<U * CH, GS, 1>(v, lane);
+#pragma unroll
+      for (int i = 0; i < OUT; ++i) {
+        const int id = sg * OUT + i;
+        s_y[r0 + id / CH][c_lane + id % CH] = v[i];
       }
     }
     __syncthreads();
@@ -126,16 +157,19 @@ __global__ void __launch_bounds__(Sh::NT) scan_forward_kernel(const ScanArgs a) 
       const int r = Share::row(i);
       const int64_t t = t0 + r;
       if (t >= stop) continue;
+      float v[V], g[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = fmaf(skip[j], to_f(cu[i].v[j]), s_y[r][col + j]);
+      if (a.z) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] = to_f(cz[i].v[j]);
+        by_two<V>(g, [](float x) { return x * sigmoid(x); }, [](float2 x) { return mul2(x, sigmoid2(x)); });
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] *= g[j];
+      }
       Chunk<T, V> o;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float v = fmaf(skip[j], to_f(cu[i].v[j]), s_y[r][col + j]);
-        if (a.z) {
-          const float zf = to_f(cz[i].v[j]);
-          v *= zf * sigmoid(zf);
-        }
-        o.v[j] = from_f<T>(t < live ? v : 0.f);
-      }
+      for (int j = 0; j < V; ++j) o.v[j] = from_f<T>(t < live ? v[j] : 0.f);
       store_chunk<T, V>(y + t * a.ys, o, left - col, a.vec);
     }
   }
@@ -149,14 +183,14 @@ __global__ void __launch_bounds__(Sh::NT) scan_forward_kernel(const ScanArgs a) 
 
   if (a.final_state && at.seg == a.segments - 1) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int n = sg * S + s;
-      if (n < a.states) {
-        float* p = a.final_state + (at.b * a.channels + cbase + c_lane) * a.states + n;
-        if (c_lane < left) p[0] = h[s].x;
-        if (c_lane + 1 < left) p[a.states] = h[s].y;
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const int n = sg * S + s;
+        if (n < a.states && c_lane + c < left)
+          a.final_state[(at.b * a.channels + cbase + c_lane + c) * a.states + n] =
+              s % 2 ? h[c].v[s / 2].y : h[c].v[s / 2].x;
       }
-    }
   }
 }
 
@@ -241,14 +275,23 @@ int bst_scan_forward(const bst_scan_desc* d, const void* u, const void* delta, c
   const int64_t per = 16 / layer_elem_size(d->dtype);
   a.vec = aligned16(u) && aligned16(delta) && aligned16(z) && aligned16(y) &&
           (a.per_group | a.ub | a.us | a.db | a.ds | (z ? a.zb | a.zs : 0) | a.yb | a.ys) % per == 0;
+  const uint64_t es = uint64_t(layer_elem_size(d->dtype));
+  auto at = [](const void* p) { return uint64_t(reinterpret_cast<uintptr_t>(p)); };
+  a.mode_act = copy_mode(at(u) | at(delta) | at(z) | es * (a.per_group | a.ub | a.us | a.db | a.ds | (z ? a.zb | a.zs : 0)));
+  a.mode_bc = copy_mode((at(B) | at(C) | es * (a.states | a.Bb | a.Bs | a.Bg | a.Cb | a.Cs | a.Cg)) % 4 ? 1 : 4);
   return with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
+    const int force = std::getenv("BST_S") ? std::atoi(std::getenv("BST_S")) : 2;
     switch (scan_pad(d->states)) {
-      case 4: return scan_forward_launch<T, ScanShape<2, 2, 4>>(a, st);
-      case 8: return scan_forward_launch<T, ScanShape<4, 2, 4>>(a, st);
-      case 16: return scan_forward_launch<T, ScanShape<4, 4, 4>>(a, st);
-      case 32: return scan_forward_launch<T, ScanShape<4, 8, 4>>(a, st);
-      default: return scan_forward_launch<T, ScanShape<4, 16, 4>>(a, st);
+      case 4: return scan_forward_launch<T, ScanShape<2, 2, 2, 2>>(a, st);
+      case 8: return scan_forward_launch<T, ScanShape<4, 2, 2, 2>>(a, st);
+      case 16:
+        if (force == 1) return scan_forward_launch<T, ScanShape<2, 1, 8, 4>>(a, st);
+        if (force == 2) return scan_forward_launch<T, ScanShape<4, 1, 4, 4>>(a, st);
+        if (force == 3) return scan_forward_launch<T, ScanShape<2, 2, 8, 4>>(a, st);
+        return scan_forward_launch<T, ScanShape<4, 2, 4, 4>>(a, st);
+      case 32: return scan_forward_launch<T, ScanShape<4, 2, 8, 4>>(a, st);
+      default: return scan_forward_launch<T, ScanShape<4, 2, 16, 4>>(a, st);
     }
   });
 }

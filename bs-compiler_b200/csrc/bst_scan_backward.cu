@@ -18,14 +18,18 @@
 
 namespace bst {
 
-template <class Sh>
+template <typename T, class Sh>
 struct BackwardShared {
-  float4 step[kScanTile][Sh::CT / 2];         // (d, d', d u, d' u') of a channel pair
-  float2 e[kScanTile][Sh::CT / 2];
-  float2 B[kScanTile][Sh::NP], C[kScanTile][Sh::NP];
-  float sum_y[kScanTile][Sh::CT];             // sum_n C h
-  float sum_g[kScanTile][Sh::CT], sum_w[kScanTile][Sh::CT];  // sum_n g B, sum_n A log2(e) w
-  float bc[Sh::W][kScanTile][2 * Sh::NP];     // per warp: dB, dC summed over its channels
+  using Share = TileShare<T, Sh>;
+  using States = StateShare<T, Sh>;
+  Step<Sh::CH> step[kScanTile][Sh::CT / Sh::CH];
+  alignas(16) float e[kScanTile][Sh::CT];
+  alignas(16) float B[kScanTile][Sh::NP], C[kScanTile][Sh::NP];
+  alignas(16) float sum_y[kScanTile][Sh::CT];                     // sum_n C h
+  float sum_g[kScanTile][Sh::CT], sum_w[kScanTile][Sh::CT];       // sum_n g B, sum_n A log2(e) w
+  float bc[Sh::W][kScanTile][2 * Sh::NP];                         // per warp: dB, dC summed over its channels
+  Chunk<T, Share::V> raw[2][4][Share::CNT][Sh::NT];               // u, delta, z, dy as they come
+  Chunk<T, States::V> raw_bc[2][2][States::CNT][Sh::NT];
 };
 
 // Sums of v over the rows of the block that share a column, by the thread of row 0.
@@ -43,16 +47,17 @@ __device__ void column_sums(float (&v)[V], float* buf) {
 
 template <typename T, class Sh>
 __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a) {
-  constexpr int S = Sh::S, GS = Sh::GS, PW = Sh::PW, CT = Sh::CT, NP = Sh::NP, NT = Sh::NT, W = Sh::W;
+  constexpr int S = Sh::S, CH = Sh::CH, GS = Sh::GS, CT = Sh::CT, NP = Sh::NP, NT = Sh::NT, W = Sh::W;
+  constexpr int LC = 32 / GS;  // lanes of a warp that share a state group
   using Share = TileShare<T, Sh>;
-  constexpr int V = Share::V, CNT = Share::CNT;
-  constexpr int BC = (kScanTile * NP + NT - 1) / NT;
+  using States = StateShare<T, Sh>;
+  constexpr int V = Share::V, CNT = Share::CNT, VB = States::V;
   extern __shared__ __align__(16) unsigned char raw_shared[];
-  BackwardShared<Sh>& m = *reinterpret_cast<BackwardShared<Sh>*>(raw_shared);
+  BackwardShared<T, Sh>& m = *reinterpret_cast<BackwardShared<T, Sh>*>(raw_shared);
 
   const ScanWhere at = scan_where(a);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int sg = lane % GS, pair = warp * PW + lane / GS;
+  const int sg = lane % GS, cell = warp * LC + lane / GS;
   const int c0 = at.ct * CT, left = a.per_group - c0;
   const int64_t cbase = int64_t(at.g) * a.per_group + c0;
   const int64_t len = scan_length(a, at.b);
@@ -60,22 +65,20 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
   const int64_t stop = min(first + int64_t(a.seg_tiles) * kScanTile, a.length);
   const int64_t live = max(min(stop, len), first);
 
-  const int c_lane = 2 * pair;
-  float2 carry[S], a2[S], dA[S];  // carry: a_{t+1} g_{t+1}
+  const int c_lane = CH * cell;
+  Pairs<S> carry[CH], a2[CH], dA[CH];  // carry: a_{t+1} g_{t+1}
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const int n = sg * S + s;
-    carry[s] = a2[s] = dA[s] = make_float2(0.f, 0.f);
-    if (n < a.states) {
-      if (c_lane < left) a2[s].x = a.A[(cbase + c_lane) * a.states + n] * kLog2e;
-      if (c_lane + 1 < left) a2[s].y = a.A[(cbase + c_lane + 1) * a.states + n] * kLog2e;
-      if (a.dfinal) {
-        const float* p = a.dfinal + (at.b * a.channels + cbase + c_lane) * a.states + n;
-        if (c_lane < left) carry[s].x = p[0];
-        if (c_lane + 1 < left) carry[s].y = p[a.states];
-      }
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int n = sg * S + s;
+      const bool on = n < a.states && c_lane + c < left;
+      const int64_t i = (cbase + c_lane + c) * a.states + n;
+      (s % 2 ? a2[c].v[s / 2].y : a2[c].v[s / 2].x) = on ? a.A[i] * kLog2e : 0.f;
+      (s % 2 ? carry[c].v[s / 2].y : carry[c].v[s / 2].x) =
+          on && a.dfinal ? a.dfinal[at.b * a.channels * a.states + i] : 0.f;
+      (s % 2 ? dA[c].v[s / 2].y : dA[c].v[s / 2].x) = 0.f;
     }
-  }
   const int col = Share::col();
   float skip[V], bias[V], dD[V], dbias[V];
 #pragma unroll
@@ -84,16 +87,10 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
     bias[i] = a.dbias && col + i < left ? a.dbias[cbase + col + i] : 0.f;
     dD[i] = dbias[i] = 0.f;
   }
-  const T* u = static_cast<const T*>(a.u) + at.b * a.ub + cbase + col;
-  const T* dl = static_cast<const T*>(a.delta) + at.b * a.db + cbase + col;
-  const T* z = static_cast<const T*>(a.z) + at.b * a.zb + cbase + col;
-  const T* dy = static_cast<const T*>(a.dy) + at.b * a.dyb + cbase + col;
   const int64_t dense = at.b * a.length * a.channels + cbase + col;  // of the contiguous gradients
   T* du = static_cast<T*>(a.du) + dense;
   T* ddl = static_cast<T*>(a.ddelta) + dense;
   T* dz = static_cast<T*>(a.dz) + dense;
-  const T* B = static_cast<const T*>(a.B) + at.b * a.Bb + at.g * a.Bg;
-  const T* C = static_cast<const T*>(a.C) + at.b * a.Cb + at.g * a.Cg;
   float* part = a.part_bc + ((at.b * a.groups + at.g) * a.col_tiles + at.ct) * a.length * 2 * NP;
 
   // Positions behind the sequence's end.
@@ -107,122 +104,170 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
     if (a.dz) store_chunk<T, V>(dz + t * a.channels, zero, left - col, a.vec);
   }
 
-  for (int64_t tile = (live - first + kScanTile - 1) / kScanTile - 1; tile >= 0; --tile) {
+  auto fetch = [&](int64_t t0, int slot) {
+    const T* u = static_cast<const T*>(a.u) + at.b * a.ub + cbase + col;
+    const T* dl = static_cast<const T*>(a.delta) + at.b * a.db + cbase + col;
+    const T* z = static_cast<const T*>(a.z) + at.b * a.zb + cbase + col;
+    const T* dy = static_cast<const T*>(a.dy) + at.b * a.dyb + cbase + col;
+    const T* B = static_cast<const T*>(a.B) + at.b * a.Bb + at.g * a.Bg;
+    const T* C = static_cast<const T*>(a.C) + at.b * a.Cb + at.g * a.Cg;
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int64_t t = t0 + Share::row(i);
+      const int n = t < live ? left - col : 0;
+      stage_chunk<T, V>(&m.raw[slot][0][i][threadIdx.x], u + t * a.us, static_cast<const T*>(a.u), n, a.mode_act);
+      stage_chunk<T, V>(&m.raw[slot][1][i][threadIdx.x], dl + t * a.ds, static_cast<const T*>(a.delta), n, a.mode_act);
+      if (a.z)
+        stage_chunk<T, V>(&m.raw[slot][2][i][threadIdx.x], z + t * a.zs, static_cast<const T*>(a.z), n, a.mode_act);
+      stage_chunk<T, V>(&m.raw[slot][3][i][threadIdx.x], dy + t * a.dys, static_cast<const T*>(a.dy), n, a.mode_act);
+    }
+#pragma unroll
+    for (int i = 0; i < States::CNT; ++i) {
+      const int k = States::item(i), n = States::state(k);
+      const int64_t t = t0 + States::row(k);
+      const int on = k < States::ITEMS && t < live ? a.states - n : 0;
+      stage_chunk<T, VB>(&m.raw_bc[slot][0][i][threadIdx.x], B + t * a.Bs + n, B, on, a.mode_bc);
+      stage_chunk<T, VB>(&m.raw_bc[slot][1][i][threadIdx.x], C + t * a.Cs + n, C, on, a.mode_bc);
+    }
+  };
+  const int64_t tiles = (live - first + kScanTile - 1) / kScanTile;
+  if (tiles > 0) fetch(first + (tiles - 1) * kScanTile, 0);
+  copy_commit();
+  int slot = 0;
+  for (int64_t tile = tiles - 1; tile >= 0; --tile, slot ^= 1) {
     const int64_t t0 = first + tile * kScanTile;
-    Chunk<T, V> cu[CNT], cd[CNT], cz[CNT], cy[CNT];
+    Pairs<S> h0[CH], h[kScanTile][CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const float* k = a.saved + ((at.b * ((a.length + kScanTile - 1) / kScanTile) + t0 / kScanTile) * a.channels +
+                                  cbase + c_lane + c) * NP + sg * S;
+      if (c_lane + c < left) h0[c] = *reinterpret_cast<const Pairs<S>*>(k);
+      else h0[c] = Pairs<S>{};
+    }
+    if (tile > 0) fetch(t0 - kScanTile, slot ^ 1);  // the next one to work on
+    copy_commit();
+    copy_wait<1>();
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
       const int r = Share::row(i);
-      const int64_t t = t0 + r;
-      const int n = t < live ? left - col : 0;
-      cu[i] = load_chunk<T, V>(u + t * a.us, n, a.vec);
-      cd[i] = load_chunk<T, V>(dl + t * a.ds, n, a.vec);
-      cz[i] = load_chunk<T, V>(z + t * a.zs, a.z ? n : 0, a.vec);
-      cy[i] = load_chunk<T, V>(dy + t * a.dys, n, a.vec);
+      const int n = t0 + r < live ? left - col : 0;
+      const Chunk<T, V> cu = m.raw[slot][0][i][threadIdx.x], cd = m.raw[slot][1][i][threadIdx.x],
+                        cz = m.raw[slot][2][i][threadIdx.x], cy = m.raw[slot][3][i][threadIdx.x];
+      float d[V], x[V], e[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = to_f(cd.v[j]) + bias[j];
+      if (a.softplus) by_two<V>(d, softplus, softplus2);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float raw = to_f(cd[i].v[j]) + bias[j];
-        const float d = j < n ? (a.softplus ? softplus(raw) : raw) : 0.f;
-        float* cell = reinterpret_cast<float*>(&m.step[r][(col + j) / 2]) + (col + j) % 2;
-        cell[0] = d;
-        cell[2] = d * to_f(cu[i].v[j]);
-        float e = to_f(cy[i].v[j]);
-        if (a.z) {
-          const float zf = to_f(cz[i].v[j]);
-          e *= zf * sigmoid(zf);
+        d[j] = j < n ? d[j] : 0.f;
+        x[j] = d[j] * to_f(cu.v[j]);
+        e[j] = to_f(cz.v[j]);
+      }
+      put_steps<CH, V>(m.step[r], col, d, x);
+      if (a.z) by_two<V>(e, [](float v) { return v * sigmoid(v); }, [](float2 v) { return mul2(v, sigmoid2(v)); });
+#pragma unroll
+      for (int j = 0; j < V; ++j) m.e[r][col + j] = a.z ? e[j] * to_f(cy.v[j]) : to_f(cy.v[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < States::CNT; ++i) {
+      const int k = States::item(i);
+      if (k < States::ITEMS) {
+        const Chunk<T, VB> cb = m.raw_bc[slot][0][i][threadIdx.x], cc = m.raw_bc[slot][1][i][threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < VB; ++j) {
+          m.B[States::row(k)][States::state(k) + j] = to_f(cb.v[j]);
+          m.C[States::row(k)][States::state(k) + j] = to_f(cc.v[j]);
         }
-        reinterpret_cast<float*>(&m.e[r][0])[col + j] = e;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < BC; ++i) {
-      const int k = threadIdx.x + i * NT, r = k / NP, n = k % NP;
-      if (r < kScanTile) {
-        const bool on = t0 + r < live && n < a.states;
-        const float vb = on ? to_f(B[(t0 + r) * a.Bs + n]) : 0.f, vc = on ? to_f(C[(t0 + r) * a.Cs + n]) : 0.f;
-        m.B[r][n] = make_float2(vb, vb);
-        m.C[r][n] = make_float2(vc, vc);
-      }
-    }
-    float2 h0[S], h[kScanTile][S];
-    {
-      const float* k = a.saved + ((at.b * ((a.length + kScanTile - 1) / kScanTile) + t0 / kScanTile) * a.channels +
-                                  cbase + c_lane) * NP + sg * S;
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-        h0[s] = make_float2(c_lane < left ? k[s] : 0.f, c_lane + 1 < left ? k[NP + s] : 0.f);
     }
     __syncthreads();
 
     // The tile's states, and sum_n C h for the gate's gradient.
-    constexpr int UY = GS >= 2 ? GS / 2 : 1;
+    constexpr int UY = GS > CH ? GS / CH : 1, OY = UY * CH / GS;
 #pragma unroll
     for (int r0 = 0; r0 < kScanTile; r0 += UY) {
-      float v[2 * UY];
+      float v[UY * CH];
 #pragma unroll
       for (int j = 0; j < UY; ++j) {
         const int r = r0 + j;
-        const float4 st = m.step[r][pair];
-        float2 acc = make_float2(0.f, 0.f);
+        const Step<CH> st = m.step[r][cell];
+        const Pairs<S> Bn = *reinterpret_cast<const Pairs<S>*>(&m.B[r][sg * S]);
+        const Pairs<S> Cn = *reinterpret_cast<const Pairs<S>*>(&m.C[r][sg * S]);
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const float2 before = r == 0 ? h0[s] : h[r > 0 ? r - 1 : 0][s];
-          const float2 x = decay(make_float2(st.x, st.y), a2[s]);
-          h[r][s] = fma2(x, before, mul2(make_float2(st.z, st.w), m.B[r][sg * S + s]));
-          acc = fma2(h[r][s], m.C[r][sg * S + s], acc);
+        for (int c = 0; c < CH; ++c) {
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int s = 0; s < S / 2; ++s) {
+            const float2 before = r == 0 ? h0[c].v[s] : h[r > 0 ? r - 1 : 0][c].v[s];
+            const float2 x = decay(both(st.d[c]), a2[c].v[s]);
+            h[r][c].v[s] = fma2(x, before, mul2(both(st.du[c]), Bn.v[s]));
+            acc = fma2(h[r][c].v[s], Cn.v[s], acc);
+          }
+          v[j * CH + c] = acc.x + acc.y;
         }
-        v[2 * j] = acc.x;
-        v[2 * j + 1] = acc.y;
       }
       if (a.z) {
-        reduce_scatter<2 * UY, GS, 1>(v, lane);
-        m.sum_y[r0 + sg / 2][c_lane + sg % 2] = v[0];
+        reduce_scatter<UY * CH, GS, 1>(v, lane);
+#pragma unroll
+        for (int i = 0; i < OY; ++i) {
+          const int id = sg * OY + i;
+          m.sum_y[r0 + id / CH][c_lane + id % CH] = v[i];
+        }
       }
     }
 
-    // Backwards.  UG steps share the sums over states (4 values a step), UB those over channels.
-    constexpr int UG = GS >= 4 ? GS / 4 : 1, NG = 4 * UG / GS;
-    constexpr int UB = 2 * S >= PW ? 1 : PW / (2 * S), NB = 2 * S * UB / PW;
+    // Backwards.  UG steps share the sums over states (2 CH values a step), UB those over channels (2 S).
+    constexpr int UG = GS > 2 * CH ? GS / (2 * CH) : 1, NG = 2 * CH * UG / GS;
+    constexpr int UB = LC > 2 * S ? LC / (2 * S) : 1, NB = 2 * S * UB / LC;
     constexpr int UU = UG > UB ? UG : UB;
 #pragma unroll
     for (int r0 = kScanTile - UU; r0 >= 0; r0 -= UU) {
-      float vg[UU][4], vb[UU][2 * S];
+      float vg[UU][2 * CH], vb[UU][2 * S];
 #pragma unroll
       for (int j = UU - 1; j >= 0; --j) {
         const int r = r0 + j;
-        const float4 st = m.step[r][pair];
-        const float2 d = make_float2(st.x, st.y), du2 = make_float2(st.z, st.w), e = m.e[r][pair];
-        float2 sg2 = make_float2(0.f, 0.f), sw2 = make_float2(0.f, 0.f);
+        const Step<CH> st = m.step[r][cell];
+        const Pairs<S> Bn = *reinterpret_cast<const Pairs<S>*>(&m.B[r][sg * S]);
+        const Pairs<S> Cn = *reinterpret_cast<const Pairs<S>*>(&m.C[r][sg * S]);
+        Pairs<S> db, dc;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const float2 Bn = m.B[r][sg * S + s], Cn = m.C[r][sg * S + s];
-          const float2 x = decay(d, a2[s]);
-          const float2 before = r == 0 ? h0[s] : h[r > 0 ? r - 1 : 0][s];
-          const float2 g = fma2(Cn, e, carry[s]);
-          const float2 w = mul2(g, mul2(x, before));
-          sw2 = fma2(w, a2[s], sw2);
-          dA[s] = fma2(w, d, dA[s]);
-          sg2 = fma2(g, Bn, sg2);
-          const float2 pb = mul2(g, du2), pc = mul2(e, h[r][s]);
-          vb[j][2 * s] = pb.x + pb.y;
-          vb[j][2 * s + 1] = pc.x + pc.y;
-          carry[s] = mul2(x, g);
+        for (int c = 0; c < CH; ++c) {
+          const float2 e = both(m.e[r][c_lane + c]), d = both(st.d[c]), x = both(st.du[c]);
+          float2 g2 = make_float2(0.f, 0.f), w2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int s = 0; s < S / 2; ++s) {
+            const float2 ex = decay(d, a2[c].v[s]);
+            const float2 before = r == 0 ? h0[c].v[s] : h[r > 0 ? r - 1 : 0][c].v[s];
+            const float2 g = fma2(Cn.v[s], e, carry[c].v[s]);
+            carry[c].v[s] = mul2(ex, g);
+            const float2 w = mul2(carry[c].v[s], before);
+            w2 = fma2(w, a2[c].v[s], w2);
+            dA[c].v[s] = fma2(w, d, dA[c].v[s]);
+            g2 = fma2(g, Bn.v[s], g2);
+            db.v[s] = c == 0 ? mul2(g, x) : fma2(g, x, db.v[s]);
+            dc.v[s] = c == 0 ? mul2(h[r][c].v[s], e) : fma2(h[r][c].v[s], e, dc.v[s]);
+          }
+          vg[j][2 * c] = g2.x + g2.y;
+          vg[j][2 * c + 1] = w2.x + w2.y;
         }
-        vg[j][0] = sg2.x;
-        vg[j][1] = sg2.y;
-        vg[j][2] = sw2.x;
-        vg[j][3] = sw2.y;
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) {
+          vb[j][2 * s] = db.v[s].x;
+          vb[j][2 * s + 1] = db.v[s].y;
+          vb[j][S + 2 * s] = dc.v[s].x;
+          vb[j][S + 2 * s + 1] = dc.v[s].y;
+        }
       }
 #pragma unroll
       for (int q = 0; q < UU / UG; ++q) {
-        float v[4 * UG];
+        float v[2 * CH * UG];
 #pragma unroll
-        for (int i = 0; i < 4 * UG; ++i) v[i] = vg[q * UG + i / 4][i % 4];
-        reduce_scatter<4 * UG, GS, 1>(v, lane);
+        for (int i = 0; i < 2 * CH * UG; ++i) v[i] = vg[q * UG + i / (2 * CH)][i % (2 * CH)];
+        reduce_scatter<2 * CH * UG, GS, 1>(v, lane);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          const int id = sg * NG + i, r = r0 + q * UG + id / 4, k = id % 4;
-          (k < 2 ? m.sum_g : m.sum_w)[r][c_lane + k % 2] = v[i];
+          const int id = sg * NG + i, r = r0 + q * UG + id / (2 * CH), k = id % (2 * CH);
+          (k % 2 ? m.sum_w : m.sum_g)[r][c_lane + k / 2] = v[i];
         }
       }
 #pragma unroll
@@ -230,11 +275,11 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
         float v[2 * S * UB];
 #pragma unroll
         for (int i = 0; i < 2 * S * UB; ++i) v[i] = vb[q * UB + i / (2 * S)][i % (2 * S)];
-        reduce_scatter<2 * S * UB, PW, GS>(v, lane);
+        reduce_scatter<2 * S * UB, LC, GS>(v, lane);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           const int id = lane / GS * NB + i, r = r0 + q * UB + id / (2 * S), k = id % (2 * S);
-          m.bc[warp][r][(k % 2) * NP + sg * S + k / 2] = v[i];
+          m.bc[warp][r][k / S * NP + sg * S + k % S] = v[i];
         }
       }
     }
@@ -245,30 +290,38 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
       const int r = Share::row(i);
       const int64_t t = t0 + r;
       if (t >= stop) continue;
+      const Chunk<T, V> cu = m.raw[slot][0][i][threadIdx.x], cd = m.raw[slot][1][i][threadIdx.x],
+                        cz = m.raw[slot][2][i][threadIdx.x], cy = m.raw[slot][3][i][threadIdx.x];
       Chunk<T, V> ou, od, oz;
+      float slope[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) slope[j] = to_f(cd.v[j]) + bias[j];
+      if (a.softplus) by_two<V>(slope, sigmoid, sigmoid2);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float uf = to_f(cu[i].v[j]), yf = to_f(cy[i].v[j]);
-        const float e = reinterpret_cast<const float*>(&m.e[r][0])[col + j];
-        const float d = (reinterpret_cast<const float*>(&m.step[r][(col + j) / 2]) + (col + j) % 2)[0];
-        const float gB = m.sum_g[r][col + j];
+        const float uf = to_f(cu.v[j]);
+        const float e = m.e[r][col + j], d = m.step[r][(col + j) / CH].d[(col + j) % CH], gB = m.sum_g[r][col + j];
         float dd = fmaf(m.sum_w[r][col + j], kLn2, gB * uf);
-        if (a.softplus) dd *= sigmoid(to_f(cd[i].v[j]) + bias[j]);
+        if (a.softplus) dd *= slope[j];
         if (t >= live) dd = 0.f;
         ou.v[j] = from_f<T>(fmaf(d, gB, skip[j] * e));
         od.v[j] = from_f<T>(dd);
         dD[j] = fmaf(e, uf, dD[j]);
         dbias[j] += dd;
-        float gz = 0.f;
-        if (a.z) {
-          const float zf = to_f(cz[i].v[j]), s = sigmoid(zf);
-          gz = yf * fmaf(skip[j], uf, m.sum_y[r][col + j]) * (s * fmaf(zf, 1.f - s, 1.f));
-        }
-        oz.v[j] = from_f<T>(gz);
       }
       store_chunk<T, V>(du + t * a.channels, ou, left - col, a.vec);
       store_chunk<T, V>(ddl + t * a.channels, od, left - col, a.vec);
-      if (a.dz) store_chunk<T, V>(dz + t * a.channels, oz, left - col, a.vec);
+      if (a.z) {
+        float s[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = to_f(cz.v[j]);
+        by_two<V>(s, sigmoid, sigmoid2);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          oz.v[j] = from_f<T>(to_f(cy.v[j]) * fmaf(skip[j], to_f(cu.v[j]), m.sum_y[r][col + j]) *
+                              (s[j] * fmaf(to_f(cz.v[j]), 1.f - s[j], 1.f)));
+        store_chunk<T, V>(dz + t * a.channels, oz, left - col, a.vec);
+      }
     }
     for (int k = threadIdx.x; k < kScanTile * 2 * NP; k += NT) {
       const int r = k / (2 * NP), n = k % (2 * NP);
@@ -282,22 +335,19 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
 
   if (a.dinit && at.seg == 0) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int n = sg * S + s;
-      if (n < a.states) {
-        float* p = a.dinit + (at.b * a.channels + cbase + c_lane) * a.states + n;
-        if (c_lane < left) p[0] = carry[s].x;
-        if (c_lane + 1 < left) p[a.states] = carry[s].y;
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const int n = sg * S + s;
+        if (n < a.states && c_lane + c < left)
+          a.dinit[(at.b * a.channels + cbase + c_lane + c) * a.states + n] =
+              s % 2 ? carry[c].v[s / 2].y : carry[c].v[s / 2].x;
       }
-    }
   }
   const int64_t prow = (at.b * a.segments + at.seg) * a.channels + cbase;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    float* p = a.part_a + (prow + c_lane) * NP + sg * S + s;
-    if (c_lane < left) p[0] = dA[s].x;
-    if (c_lane + 1 < left) p[NP] = dA[s].y;
-  }
+  for (int c = 0; c < CH; ++c)
+    if (c_lane + c < left) *reinterpret_cast<Pairs<S>*>(a.part_a + (prow + c_lane + c) * NP + sg * S) = dA[c];
   float* buf = &m.sum_y[0][0];  // sum_y, sum_g and sum_w: 48 CT floats for NT V = 16 CT / CNT
   column_sums<Sh, V, Share::PER_ROW>(dD, buf);
   column_sums<Sh, V, Share::PER_ROW>(dbias, buf);
@@ -355,11 +405,11 @@ __global__ void __launch_bounds__(256) scan_params_kernel(const ScanArgs a, int 
 template <class F>
 static auto with_backward_shape(int64_t states, F&& f) {
   switch (scan_pad(states)) {
-    case 4: return f(ScanShape<2, 2, 4>{});
-    case 8: return f(ScanShape<2, 4, 4>{});
-    case 16: return f(ScanShape<2, 8, 8>{});
-    case 32: return f(ScanShape<2, 16, 8>{});
-    default: return f(ScanShape<2, 32, 8>{});
+    case 4: return f(ScanShape<2, 2, 2, 2>{});
+    case 8: return f(ScanShape<4, 2, 2, 2>{});
+    case 16: return f(ScanShape<4, 2, 4, 4>{});
+    case 32: return f(ScanShape<4, 2, 8, 4>{});
+    default: return f(ScanShape<4, 2, 16, 4>{});
   }
 }
 
@@ -386,7 +436,7 @@ static int scan_backward_launch(ScanArgs a, cudaStream_t st) {
   const int64_t outs = int64_t(a.batch) * a.length * a.groups * 2 * Sh::NP;
   if (blocks > INT_MAX || outs / 256 + 1 > INT_MAX)
     return fail(BST_ERR_UNSUPPORTED, "the scan's gradients need more than 2^31 blocks");
-  constexpr int smem = int(sizeof(BackwardShared<Sh>));
+  constexpr int smem = int(sizeof(BackwardShared<T, Sh>));
   auto* kernel = scan_backward_kernel<T, Sh>;
   BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kernel<<<unsigned(blocks), Sh::NT, smem, st>>>(a);
@@ -436,6 +486,11 @@ extern "C" int bst_scan_backward(const bst_scan_desc* d, const void* u, const vo
   a.vec = aligned16(u) && aligned16(delta) && aligned16(z) && aligned16(dy) && aligned16(du) && aligned16(ddelta) &&
           aligned16(dz) &&
           (a.per_group | a.ub | a.us | a.db | a.ds | (z ? a.zb | a.zs : 0) | a.dyb | a.dys) % per == 0;
+  const uint64_t es = uint64_t(layer_elem_size(d->dtype));
+  auto at = [](const void* p) { return uint64_t(reinterpret_cast<uintptr_t>(p)); };
+  a.mode_act = copy_mode(at(u) | at(delta) | at(z) | at(dy) |
+                         es * (a.per_group | a.ub | a.us | a.db | a.ds | (z ? a.zb | a.zs : 0) | a.dyb | a.dys));
+  a.mode_bc = copy_mode((at(B) | at(C) | es * (a.states | a.Bb | a.Bs | a.Bg | a.Cb | a.Cs | a.Cg)) % 4 ? 1 : 4);
   int rc = with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
     return with_backward_shape(d->states, [&](auto sh) { return scan_backward_launch<T, decltype(sh)>(a, st); });
