@@ -12,6 +12,12 @@
 // steps: a block loads a tile of u, delta (z, dy) for its channels and of B, C, computes what is shared
 // by the states (the step size) once, and leaves it in shared memory as the steps want it.
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <type_traits>
+
+#include "bst_kernels.cuh"  // mbarrier helpers
 #include "bst_layer.cuh"
 
 namespace bst {
@@ -31,7 +37,8 @@ struct ScanArgs {
   int64_t length;
   int channels, per_group, groups, states, batch;
   int softplus, vec;
-  int mode_act, mode_bc;  // CopyMode of the activations, of B and C
+  int mode;         // CopyMode of the inputs
+  unsigned* error;  // the device's error word
   int segments, seg_tiles, col_tiles;  // segments per sequence, 16-step tiles per segment, channel tiles per group
 };
 
@@ -68,38 +75,57 @@ __device__ __forceinline__ ScanWhere scan_where(const ScanArgs& a) {
   return w;
 }
 
-// A thread's share of a [16 x CT] tile of an activation: CNT chunks of V elements, chunk i at row
-// row(i), column col (the same for all of them).
-template <typename T, class Sh>
-struct TileShare {
-  static constexpr int E = kScanTile * Sh::CT / Sh::NT;
-  static constexpr int VMAX = 16 / int(sizeof(T));
-  static constexpr int V = E < VMAX ? E : VMAX;
-  static constexpr int CNT = E / V;
-  static constexpr int PER_ROW = Sh::CT / V;
-  static constexpr int ROWS = Sh::NT / PER_ROW;  // rows covered by one round of the block
-  static_assert(Sh::NT % PER_ROW == 0 && ROWS * CNT == kScanTile, "a round covers whole rows");
-  __device__ static int row(int i) { return i * ROWS + int(threadIdx.x) / PER_ROW; }
-  __device__ static int col() { return (int(threadIdx.x) % PER_ROW) * V; }
+// A helper thread's share of a [16 x CT] tile: pairs of neighbouring channels, lane by lane along a row, so that
+// its accesses to shared memory and to the outputs are contiguous across a warp.  TURNS rows per thread, ROWS apart.
+// A block has as many helper threads as recurrence threads; they come second.
+template <class Sh>
+struct PairShare {
+  static constexpr int PAIRS = Sh::CT / 2;
+  static constexpr int ROWS = Sh::NT / PAIRS;
+  static constexpr int TURNS = kScanTile / ROWS;
+  static_assert(Sh::NT % PAIRS == 0 && ROWS * TURNS == kScanTile, "a turn covers whole rows");
+  __device__ static int me() { return int(threadIdx.x) - Sh::NT; }
+  __device__ static int row(int i) { return i * ROWS + me() / PAIRS; }
+  __device__ static int col() { return me() % PAIRS * 2; }
 };
 
+// Barriers of a block's two halves, two of each (one per buffer): one half arrives, the other waits.  Their numbers
+// are immediates, so that the block does not reserve all sixteen.
+enum ScanBarrier : int { kFull = 1, kDone = 3, kHelp = 5 };  // kHelp: among the helpers
+template <int THREADS, int ID>
+__device__ __forceinline__ void bar_sync(int buf) {
+  if (buf) asm volatile("bar.sync %0, %1;" ::"n"(ID + 1), "n"(THREADS) : "memory");
+  else asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(THREADS) : "memory");
+}
+template <int THREADS, int ID>
+__device__ __forceinline__ void bar_arrive(int buf) {
+  if (buf) asm volatile("bar.arrive %0, %1;" ::"n"(ID + 1), "n"(THREADS) : "memory");
+  else asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(THREADS) : "memory");
+}
+
 // ---- asynchronous copies of a tile's inputs ------------------------------------------
-// Each thread copies its own share of a tile into slots of shared memory that only it reads, so that a
-// wait for its own copies is all the ordering they need.  How a tensor can be copied:
+// How the inputs can be copied (by the alignment of their bases and strides):
 enum CopyMode : int {
   kCopyPlain = 0,  // element by element through registers (2-byte elements at odd distances)
   kCopyWords = 1,  // 4 bytes at a time
-  kCopyChunk = 2   // whole chunks
+  kCopyTiles = 2   // whole tiles, by the tensor copy engine (16-byte alignment)
 };
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from, bool on) {
-  const unsigned dst = unsigned(__cvta_generic_to_shared(to));
-  const int n = on ? BYTES : 0;  // the rest of the destination is filled with zeros
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(from), "r"(n), "n"(BYTES) : "memory");
+__device__ __forceinline__ void copy_async4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+// The inputs as the tensor copy engine sees them: [batch, length, channels] in boxes of 16 positions, and
+// [batch, length, groups, states].  What lies outside of a tensor reads zero.
+struct ScanMaps {
+  CUtensorMap u, delta, z, dy, B, C;
+};
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
@@ -107,81 +133,67 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
-// Elements [0, n) of src (the others zero) into a chunk of shared memory.  `base`: any valid address.
-template <typename T, int V>
-__device__ __forceinline__ void stage_chunk(Chunk<T, V>* dst, const T* src, const T* base, int n, int mode) {
-  constexpr int BYTES = int(sizeof(T)) * V, PER = 4 / int(sizeof(T));
-  if constexpr (BYTES >= 4) {
-    if (mode == kCopyChunk) {
-      copy_async<BYTES>(dst, n >= V ? src : base, n >= V);
-      return;
-    }
-    if (mode == kCopyWords) {
-#pragma unroll
-      for (int j = 0; j < V; j += PER) copy_async<4>(&dst->v[j], j < n ? src + j : base, j < n);
-      return;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) dst->v[j] = j < n ? src[j] : from_f<T>(0.f);
-}
-
-// B and C of a tile: pairs of neighbouring states (single ones in fp32), BC of them per thread.
-template <typename T, class Sh>
-struct StateShare {
-  static constexpr int V = 4 / int(sizeof(T));
-  static constexpr int ITEMS = kScanTile * Sh::NP / V;
-  static constexpr int CNT = (ITEMS + Sh::NT - 1) / Sh::NT;
-  __device__ static int item(int i) { return int(threadIdx.x) + i * Sh::NT; }
-  __device__ static int row(int k) { return k / (Sh::NP / V); }
-  __device__ static int state(int k) { return k % (Sh::NP / V) * V; }
-};
-
-// a_t of two states; a2 = A log2(e).
-__device__ __forceinline__ float2 decay(float2 step, float2 a2) { return ex2_2(mul2(step, a2)); }
-
 // S consecutive floats, as pairs.
 template <int S>
 struct alignas(4 * S) Pairs {
   float2 v[S / 2];
 };
+// The first `cols` columns of `rows` rows of a [16 x WIDTH] tile, from rows `step` apart, by NT threads of which this
+// one is `me`, in words or elements.  The other columns are filled with zeros, the other rows left as they were.
+template <typename T, int WIDTH, int NT>
+__device__ __forceinline__ void stage_tile(T* to, const T* from, int64_t step, int rows, int cols, bool words, int me) {
+  constexpr int P = 4 / int(sizeof(T)), ACROSS = WIDTH / P;
+  if (words) {
+    for (int k = me; k < rows * ACROSS; k += NT) {
+      const int r = k / ACROSS, c = k % ACROSS * P;
+      if (c < cols) copy_async4(to + r * WIDTH + c, from + r * step + c);
+      else *reinterpret_cast<uint32_t*>(to + r * WIDTH + c) = 0;
+    }
+  } else {
+    for (int k = me; k < rows * WIDTH; k += NT) {
+      const int r = k / WIDTH, c = k % WIDTH;
+      to[k] = c < cols ? from[r * step + c] : from_f<T>(0.f);
+    }
+  }
+}
+
+// S states of a tile of B or C, as fp32 pairs.
+template <int S, typename T>
+__device__ __forceinline__ Pairs<S> load_states(const T* p) {
+  const Chunk<T, S> c = *reinterpret_cast<const Chunk<T, S>*>(p);
+  Pairs<S> r;
+#pragma unroll
+  for (int i = 0; i < S / 2; ++i) r.v[i] = make_float2(to_f(c.v[2 * i]), to_f(c.v[2 * i + 1]));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 load_pair(const T* p) {
+  const Chunk<T, 2> c = *reinterpret_cast<const Chunk<T, 2>*>(p);
+  return make_float2(to_f(c.v[0]), to_f(c.v[1]));
+}
+template <typename T>
+__device__ __forceinline__ Chunk<T, 2> to_pair(float2 v) {
+  Chunk<T, 2> c;
+  c.v[0] = from_f<T>(v.x);
+  c.v[1] = from_f<T>(v.y);
+  return c;
+}
+
+// a_t of two states; a2 = A log2(e).
+__device__ __forceinline__ float2 decay(float2 step, float2 a2) { return ex2_2(mul2(step, a2)); }
+
 // What the states of CH neighbouring channels share at one step.
 template <int CH>
 struct alignas(8 * CH) Step {
   float d[CH], du[CH];
 };
 
-// Step sizes d and d u of a thread's chunk of V channels, into the tile's shared memory.
-template <int CH, int V>
-__device__ __forceinline__ void put_steps(Step<CH>* row, int col, const float (&d)[V], const float (&du)[V]) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if constexpr (CH == 2 && V % 2 == 0) {
-      if (j % 2 == 0) {
-        Step<2> s;
-        s.d[0] = d[j], s.d[1] = d[j + 1], s.du[0] = du[j], s.du[1] = du[j + 1];
-        row[(col + j) / 2] = s;
-      }
-    } else {
-      row[(col + j) / CH].d[(col + j) % CH] = d[j];
-      row[(col + j) / CH].du[(col + j) % CH] = du[j];
-    }
-  }
-}
-
-// v -> f2 of neighbouring values (f1 of a single one).
-template <int V, class F1, class F2>
-__device__ __forceinline__ void by_two(float (&v)[V], F1&& f1, F2&& f2) {
-  if constexpr (V == 1) {
-    v[0] = f1(v[0]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; j += 2) {
-      const float2 r = f2(make_float2(v[j], v[j + 1]));
-      v[j] = r.x;
-      v[j + 1] = r.y;
-    }
-  }
+// Step sizes d and d u of a pair of channels (col even), into a row of the tile's shared memory.
+template <int CH>
+__device__ __forceinline__ void put_steps(Step<CH>* row, int col, float2 d, float2 du) {
+  if constexpr (CH == 2) *reinterpret_cast<float4*>(&row[col / 2]) = make_float4(d.x, d.y, du.x, du.y);
+  else *reinterpret_cast<float4*>(&row[col]) = make_float4(d.x, du.x, d.y, du.y);
 }
 
 // Host: states per lane and the group count for N states.
@@ -191,8 +203,11 @@ inline int scan_pad(int64_t n) {
   return p;
 }
 
-// How activations whose base pointers and strides are or-ed into `bits` (in bytes) can be copied.
-inline int copy_mode(uint64_t bits) { return bits % 16 == 0 ? kCopyChunk : bits % 4 == 0 ? kCopyWords : kCopyPlain; }
+int scan_copy_mode(const bst_scan_desc* d, const void* u, const void* delta, const void* z, const void* dy,
+                   const void* B, const void* C);
+// Tensor maps of a scan's inputs; false where they cannot be made (the words path then copies).
+bool scan_maps(const bst_scan_desc* d, int tile_channels, int pad, const void* u, const void* delta, const void* z,
+               const void* dy, const void* B, const void* C, ScanMaps* m);
 
 int scan_check(const bst_scan_desc* d);
 ScanArgs scan_args(const bst_scan_desc* d);

@@ -20,50 +20,34 @@ namespace bst {
 
 template <typename T, class Sh>
 struct BackwardShared {
-  using Share = TileShare<T, Sh>;
-  using States = StateShare<T, Sh>;
-  Step<Sh::CH> step[kScanTile][Sh::CT / Sh::CH];
-  alignas(16) float e[kScanTile][Sh::CT];
-  alignas(16) float B[kScanTile][Sh::NP], C[kScanTile][Sh::NP];
+  alignas(128) T act[2][4][kScanTile][Sh::CT];                    // u, delta, dy, z as they come: this tile, the next
+  alignas(128) T bc[2][2][kScanTile][Sh::NP];                     // B, C
+  alignas(16) float d[kScanTile][Sh::CT], e[kScanTile][Sh::CT];   // step sizes, gradients of the sums over states
   alignas(16) float sum_y[kScanTile][Sh::CT];                     // sum_n C h
   float sum_g[kScanTile][Sh::CT], sum_w[kScanTile][Sh::CT];       // sum_n g B, sum_n A log2(e) w
-  float bc[Sh::W][kScanTile][2 * Sh::NP];                         // per warp: dB, dC summed over its channels
-  Chunk<T, Share::V> raw[2][4][Share::CNT][Sh::NT];               // u, delta, z, dy as they come
-  Chunk<T, States::V> raw_bc[2][2][States::CNT][Sh::NT];
+  float part[Sh::W][kScanTile][2 * Sh::NP];                       // per warp: dB, dC summed over its channels
+  uint64_t bar[2];
 };
 
-// Sums of v over the rows of the block that share a column, by the thread of row 0.
-template <class Sh, int V, int PER_ROW>
-__device__ void column_sums(float (&v)[V], float* buf) {
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < V; ++j) buf[threadIdx.x * V + j] = v[j];
-  __syncthreads();
-  if (threadIdx.x < PER_ROW)
-    for (int r = 1; r < Sh::NT / PER_ROW; ++r)
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] += buf[(threadIdx.x + r * PER_ROW) * V + j];
-}
-
-template <typename T, class Sh>
-__global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a) {
+template <typename T, class Sh, bool TILES>
+__global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
+                                                               const __grid_constant__ ScanMaps maps) {
   constexpr int S = Sh::S, CH = Sh::CH, GS = Sh::GS, CT = Sh::CT, NP = Sh::NP, NT = Sh::NT, W = Sh::W;
   constexpr int LC = 32 / GS;  // lanes of a warp that share a state group
-  using Share = TileShare<T, Sh>;
-  using States = StateShare<T, Sh>;
-  constexpr int V = Share::V, CNT = Share::CNT, VB = States::V;
-  extern __shared__ __align__(16) unsigned char raw_shared[];
+  constexpr int PAIRS = CT / 2, ROWS = NT / PAIRS, TURNS = kScanTile / ROWS;
+  extern __shared__ __align__(128) unsigned char raw_shared[];
   BackwardShared<T, Sh>& m = *reinterpret_cast<BackwardShared<T, Sh>*>(raw_shared);
 
   const ScanWhere at = scan_where(a);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int sg = lane % GS, cell = warp * LC + lane / GS;
-  const int c0 = at.ct * CT, left = a.per_group - c0;
+  const int c0 = at.ct * CT, left = a.per_group - c0, cols = left < CT ? left : CT;
   const int64_t cbase = int64_t(at.g) * a.per_group + c0;
   const int64_t len = scan_length(a, at.b);
   const int64_t first = int64_t(at.seg) * a.seg_tiles * kScanTile;
   const int64_t stop = min(first + int64_t(a.seg_tiles) * kScanTile, a.length);
   const int64_t live = max(min(stop, len), first);
+  const int tiles = int((live - first + kScanTile - 1) / kScanTile);
 
   const int c_lane = CH * cell;
   Pairs<S> carry[CH], a2[CH], dA[CH];  // carry: a_{t+1} g_{t+1}
@@ -79,14 +63,12 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
           on && a.dfinal ? a.dfinal[at.b * a.channels * a.states + i] : 0.f;
       (s % 2 ? dA[c].v[s / 2].y : dA[c].v[s / 2].x) = 0.f;
     }
-  const int col = Share::col();
-  float skip[V], bias[V], dD[V], dbias[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    skip[i] = a.D && col + i < left ? a.D[cbase + col + i] : 0.f;
-    bias[i] = a.dbias && col + i < left ? a.dbias[cbase + col + i] : 0.f;
-    dD[i] = dbias[i] = 0.f;
-  }
+  // Outside of the recurrences a thread has a pair of neighbouring channels and every ROWS-th position.
+  const int col = threadIdx.x % PAIRS * 2, row0 = threadIdx.x / PAIRS;
+  const bool in0 = col < left, in1 = col + 1 < left;
+  float2 skip = both(0.f), bias = both(0.f), dD = both(0.f), dbias = both(0.f);
+  if (a.D) skip = make_float2(in0 ? a.D[cbase + col] : 0.f, in1 ? a.D[cbase + col + 1] : 0.f);
+  if (a.dbias) bias = make_float2(in0 ? a.dbias[cbase + col] : 0.f, in1 ? a.dbias[cbase + col + 1] : 0.f);
   const int64_t dense = at.b * a.length * a.channels + cbase + col;  // of the contiguous gradients
   T* du = static_cast<T*>(a.du) + dense;
   T* ddl = static_cast<T*>(a.ddelta) + dense;
@@ -94,156 +76,203 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
   float* part = a.part_bc + ((at.b * a.groups + at.g) * a.col_tiles + at.ct) * a.length * 2 * NP;
 
   // Positions behind the sequence's end.
-  Chunk<T, V> zero;
-#pragma unroll
-  for (int j = 0; j < V; ++j) zero.v[j] = from_f<T>(0.f);
-  for (int64_t t = (live + kScanTile - 1) / kScanTile * kScanTile + int(threadIdx.x) / Share::PER_ROW; t < stop;
-       t += Share::ROWS) {
-    store_chunk<T, V>(du + t * a.channels, zero, left - col, a.vec);
-    store_chunk<T, V>(ddl + t * a.channels, zero, left - col, a.vec);
-    if (a.dz) store_chunk<T, V>(dz + t * a.channels, zero, left - col, a.vec);
+  for (int64_t t = first + int64_t(tiles) * kScanTile + row0; t < stop; t += ROWS) {
+    const Chunk<T, 2> zero = to_pair<T>(both(0.f));
+    store_chunk<T, 2>(du + t * a.channels, zero, left - col, a.vec);
+    store_chunk<T, 2>(ddl + t * a.channels, zero, left - col, a.vec);
+    if (a.dz) store_chunk<T, 2>(dz + t * a.channels, zero, left - col, a.vec);
   }
 
-  auto fetch = [&](int64_t t0, int slot) {
-    const T* u = static_cast<const T*>(a.u) + at.b * a.ub + cbase + col;
-    const T* dl = static_cast<const T*>(a.delta) + at.b * a.db + cbase + col;
-    const T* z = static_cast<const T*>(a.z) + at.b * a.zb + cbase + col;
-    const T* dy = static_cast<const T*>(a.dy) + at.b * a.dyb + cbase + col;
-    const T* B = static_cast<const T*>(a.B) + at.b * a.Bb + at.g * a.Bg;
-    const T* C = static_cast<const T*>(a.C) + at.b * a.Cb + at.g * a.Cg;
-#pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int64_t t = t0 + Share::row(i);
-      const int n = t < live ? left - col : 0;
-      stage_chunk<T, V>(&m.raw[slot][0][i][threadIdx.x], u + t * a.us, static_cast<const T*>(a.u), n, a.mode_act);
-      stage_chunk<T, V>(&m.raw[slot][1][i][threadIdx.x], dl + t * a.ds, static_cast<const T*>(a.delta), n, a.mode_act);
-      if (a.z)
-        stage_chunk<T, V>(&m.raw[slot][2][i][threadIdx.x], z + t * a.zs, static_cast<const T*>(a.z), n, a.mode_act);
-      stage_chunk<T, V>(&m.raw[slot][3][i][threadIdx.x], dy + t * a.dys, static_cast<const T*>(a.dy), n, a.mode_act);
+  bool failed = false;
+  if (TILES) {
+    if (threadIdx.x == 0) {
+      mbar_init(&m.bar[0], 1);
+      mbar_init(&m.bar[1], 1);
+      mbar_fence_init();
     }
-#pragma unroll
-    for (int i = 0; i < States::CNT; ++i) {
-      const int k = States::item(i), n = States::state(k);
-      const int64_t t = t0 + States::row(k);
-      const int on = k < States::ITEMS && t < live ? a.states - n : 0;
-      stage_chunk<T, VB>(&m.raw_bc[slot][0][i][threadIdx.x], B + t * a.Bs + n, B, on, a.mode_bc);
-      stage_chunk<T, VB>(&m.raw_bc[slot][1][i][threadIdx.x], C + t * a.Cs + n, C, on, a.mode_bc);
+    __syncthreads();
+  }
+  auto fetch = [&](int k, int slot) {
+    if (k >= 0) {
+      auto& act = m.act[slot];
+      auto& bc = m.bc[slot];
+      const int64_t t0 = first + int64_t(k) * kScanTile;
+      if constexpr (TILES) {
+        if (threadIdx.x == 0) {
+          uint64_t* bar = &m.bar[slot];
+          const int t = int(t0), c = int(cbase), b = int(at.b);
+          mbar_expect_tx(bar, unsigned((a.z ? 4 : 3) * sizeof(act[0]) + sizeof(bc)));
+          tma_load_3d(&act[0][0][0], &maps.u, bar, c, t, b);
+          tma_load_3d(&act[1][0][0], &maps.delta, bar, c, t, b);
+          tma_load_3d(&act[2][0][0], &maps.dy, bar, c, t, b);
+          if (a.z) tma_load_3d(&act[3][0][0], &maps.z, bar, c, t, b);
+          tma_load_4d(&bc[0][0][0], &maps.B, bar, 0, at.g, t, b);
+          tma_load_4d(&bc[1][0][0], &maps.C, bar, 0, at.g, t, b);
+        }
+      } else {
+        const int rows = int(min(live - t0, int64_t(kScanTile))), me = threadIdx.x;
+        const bool words = a.mode == kCopyWords;
+        auto stage = [&](auto width, T* to, const void* p, int64_t off, int64_t st, int n) {
+          stage_tile<T, decltype(width)::value, NT>(to, static_cast<const T*>(p) + off + t0 * st, st, rows, n, words, me);
+        };
+        std::integral_constant<int, CT> wide;
+        std::integral_constant<int, NP> slim;
+        stage(wide, &act[0][0][0], a.u, at.b * a.ub + cbase, a.us, cols);
+        stage(wide, &act[1][0][0], a.delta, at.b * a.db + cbase, a.ds, cols);
+        stage(wide, &act[2][0][0], a.dy, at.b * a.dyb + cbase, a.dys, cols);
+        if (a.z) stage(wide, &act[3][0][0], a.z, at.b * a.zb + cbase, a.zs, cols);
+        stage(slim, &bc[0][0][0], a.B, at.b * a.Bb + at.g * a.Bg, a.Bs, a.states);
+        stage(slim, &bc[1][0][0], a.C, at.b * a.Cb + at.g * a.Cg, a.Cs, a.states);
+      }
     }
+    if constexpr (!TILES) copy_commit();
   };
-  const int64_t tiles = (live - first + kScanTile - 1) / kScanTile;
-  if (tiles > 0) fetch(first + (tiles - 1) * kScanTile, 0);
-  copy_commit();
-  int slot = 0;
-  for (int64_t tile = tiles - 1; tile >= 0; --tile, slot ^= 1) {
-    const int64_t t0 = first + tile * kScanTile;
+  fetch(tiles - 1, 0);
+  int slot = 0, turn = 0;
+  for (int k = tiles - 1; k >= 0; --k) {
+    const int64_t t0 = first + int64_t(k) * kScanTile;
+    const int rows = int(min(live - t0, int64_t(kScanTile)));
     Pairs<S> h0[CH], h[kScanTile][CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const float* k = a.saved + ((at.b * ((a.length + kScanTile - 1) / kScanTile) + t0 / kScanTile) * a.channels +
+      const float* p = a.saved + ((at.b * ((a.length + kScanTile - 1) / kScanTile) + t0 / kScanTile) * a.channels +
                                   cbase + c_lane + c) * NP + sg * S;
-      if (c_lane + c < left) h0[c] = *reinterpret_cast<const Pairs<S>*>(k);
+      if (c_lane + c < left) h0[c] = *reinterpret_cast<const Pairs<S>*>(p);
       else h0[c] = Pairs<S>{};
     }
-    if (tile > 0) fetch(t0 - kScanTile, slot ^ 1);  // the next one to work on
-    copy_commit();
-    copy_wait<1>();
-#pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int r = Share::row(i);
-      const int n = t0 + r < live ? left - col : 0;
-      const Chunk<T, V> cu = m.raw[slot][0][i][threadIdx.x], cd = m.raw[slot][1][i][threadIdx.x],
-                        cz = m.raw[slot][2][i][threadIdx.x], cy = m.raw[slot][3][i][threadIdx.x];
-      float d[V], x[V], e[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = to_f(cd.v[j]) + bias[j];
-      if (a.softplus) by_two<V>(d, softplus, softplus2);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        d[j] = j < n ? d[j] : 0.f;
-        x[j] = d[j] * to_f(cu.v[j]);
-        e[j] = to_f(cz.v[j]);
+    fetch(k - 1, slot ^ 1);  // the next tile to work on
+    if constexpr (TILES) {
+      if (!failed && !mbar_wait_bounded(&m.bar[slot], unsigned(turn) & 1u)) {
+        failed = true;
+        atomicOr(a.error, kErrTmaTimeout);
       }
-      put_steps<CH, V>(m.step[r], col, d, x);
-      if (a.z) by_two<V>(e, [](float v) { return v * sigmoid(v); }, [](float2 v) { return mul2(v, sigmoid2(v)); });
-#pragma unroll
-      for (int j = 0; j < V; ++j) m.e[r][col + j] = a.z ? e[j] * to_f(cy.v[j]) : to_f(cy.v[j]);
+    } else {
+      copy_wait<1>();
+      __syncthreads();  // everybody's copies
     }
+    auto& act = m.act[slot];
+    {
+      float2 d[TURNS], e[TURNS];
 #pragma unroll
-    for (int i = 0; i < States::CNT; ++i) {
-      const int k = States::item(i);
-      if (k < States::ITEMS) {
-        const Chunk<T, VB> cb = m.raw_bc[slot][0][i][threadIdx.x], cc = m.raw_bc[slot][1][i][threadIdx.x];
+      for (int i = 0; i < TURNS; ++i) {
+        d[i] = add2(load_pair(&act[1][row0 + i * ROWS][col]), bias);
+        e[i] = load_pair(&act[2][row0 + i * ROWS][col]);
+      }
+      if (a.softplus) {
 #pragma unroll
-        for (int j = 0; j < VB; ++j) {
-          m.B[States::row(k)][States::state(k) + j] = to_f(cb.v[j]);
-          m.C[States::row(k)][States::state(k) + j] = to_f(cc.v[j]);
+        for (int i = 0; i < TURNS; ++i) d[i] = softplus2(d[i]);
+      }
+      if (a.z) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+          const float2 z = load_pair(&act[3][row0 + i * ROWS][col]);
+          e[i] = mul2(e[i], mul2(z, sigmoid2(z)));
         }
+      }
+      if (rows < kScanTile) {  // what lies behind the sequence's end may be anything: it becomes zeros
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i)
+          if (row0 + i * ROWS >= rows) {
+            d[i] = e[i] = both(0.f);
+            *reinterpret_cast<Chunk<T, 2>*>(&act[0][row0 + i * ROWS][col]) = to_pair<T>(both(0.f));
+          }
+        for (int j = rows * NP + int(threadIdx.x); j < kScanTile * NP; j += NT)
+          (&m.bc[slot][0][0][0])[j] = (&m.bc[slot][1][0][0])[j] = from_f<T>(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        *reinterpret_cast<float2*>(&m.d[row0 + i * ROWS][col]) = d[i];
+        *reinterpret_cast<float2*>(&m.e[row0 + i * ROWS][col]) = e[i];
       }
     }
     __syncthreads();
 
-    // The tile's states, and sum_n C h for the gate's gradient.
+    // What a step of the recurrences reads.
+    struct Operands {
+      Chunk<float, CH> d, e;
+      Chunk<T, CH> u;
+      Chunk<T, S> B, C;
+    };
+    auto load = [&](int r) {
+      Operands o;
+      o.d = *reinterpret_cast<const Chunk<float, CH>*>(&m.d[r][c_lane]);
+      o.e = *reinterpret_cast<const Chunk<float, CH>*>(&m.e[r][c_lane]);
+      o.u = *reinterpret_cast<const Chunk<T, CH>*>(&act[0][r][c_lane]);
+      o.B = *reinterpret_cast<const Chunk<T, S>*>(&m.bc[slot][0][r][sg * S]);
+      o.C = *reinterpret_cast<const Chunk<T, S>*>(&m.bc[slot][1][r][sg * S]);
+      return o;
+    };
+    // The tile's states, and sum_n C h for the gate's gradient (left in registers until the loop is over: a store
+    // in between would hold back the loads of the later steps).
     constexpr int UY = GS > CH ? GS / CH : 1, OY = UY * CH / GS;
+    float sums[kScanTile / UY][OY];
 #pragma unroll
     for (int r0 = 0; r0 < kScanTile; r0 += UY) {
       float v[UY * CH];
 #pragma unroll
       for (int j = 0; j < UY; ++j) {
         const int r = r0 + j;
-        const Step<CH> st = m.step[r][cell];
-        const Pairs<S> Bn = *reinterpret_cast<const Pairs<S>*>(&m.B[r][sg * S]);
-        const Pairs<S> Cn = *reinterpret_cast<const Pairs<S>*>(&m.C[r][sg * S]);
+        const Operands o = load(r);
+        const Pairs<S> Bn = load_states<S>(o.B.v), Cn = load_states<S>(o.C.v);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
+          const float x = o.d.v[c] * to_f(o.u.v[c]);
           float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
           for (int s = 0; s < S / 2; ++s) {
             const float2 before = r == 0 ? h0[c].v[s] : h[r > 0 ? r - 1 : 0][c].v[s];
-            const float2 x = decay(both(st.d[c]), a2[c].v[s]);
-            h[r][c].v[s] = fma2(x, before, mul2(both(st.du[c]), Bn.v[s]));
-            acc = fma2(h[r][c].v[s], Cn.v[s], acc);
+            h[r][c].v[s] = fma2(decay(both(o.d.v[c]), a2[c].v[s]), before, mul2(both(x), Bn.v[s]));
+            acc = s == 0 ? mul2(h[r][c].v[s], Cn.v[s]) : fma2(h[r][c].v[s], Cn.v[s], acc);
           }
           v[j * CH + c] = acc.x + acc.y;
         }
       }
-      if (a.z) {
-        reduce_scatter<UY * CH, GS, 1>(v, lane);
+      if (a.z) reduce_scatter<UY * CH, GS, 1>(v, lane);
+#pragma unroll
+      for (int i = 0; i < OY; ++i) sums[r0 / UY][i] = v[i];
+    }
+    if (a.z) {
+#pragma unroll
+      for (int r0 = 0; r0 < kScanTile; r0 += UY)
 #pragma unroll
         for (int i = 0; i < OY; ++i) {
           const int id = sg * OY + i;
-          m.sum_y[r0 + id / CH][c_lane + id % CH] = v[i];
+          m.sum_y[r0 + id / CH][c_lane + id % CH] = sums[r0 / UY][i];
         }
-      }
     }
 
-    // Backwards.  UG steps share the sums over states (2 CH values a step), UB those over channels (2 S).
+    // Backwards.  UG steps share the sums over states (2 CH values a step), UB those over channels (2 S).  The
+    // operands are loaded AHEAD steps early, past the stores of the steps in between.
     constexpr int UG = GS > 2 * CH ? GS / (2 * CH) : 1, NG = 2 * CH * UG / GS;
     constexpr int UB = LC > 2 * S ? LC / (2 * S) : 1, NB = 2 * S * UB / LC;
     constexpr int UU = UG > UB ? UG : UB;
+    constexpr int AHEAD = UU > 2 ? UU : 2;
+    Operands next[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) next[j] = load(kScanTile - 1 - j);
 #pragma unroll
     for (int r0 = kScanTile - UU; r0 >= 0; r0 -= UU) {
       float vg[UU][2 * CH], vb[UU][2 * S];
 #pragma unroll
       for (int j = UU - 1; j >= 0; --j) {
         const int r = r0 + j;
-        const Step<CH> st = m.step[r][cell];
-        const Pairs<S> Bn = *reinterpret_cast<const Pairs<S>*>(&m.B[r][sg * S]);
-        const Pairs<S> Cn = *reinterpret_cast<const Pairs<S>*>(&m.C[r][sg * S]);
+        const Operands o = next[(kScanTile - 1 - r) % AHEAD];
+        if (r >= AHEAD) next[(kScanTile - 1 - r) % AHEAD] = load(r - AHEAD);
+        const Pairs<S> Bn = load_states<S>(o.B.v), Cn = load_states<S>(o.C.v);
         Pairs<S> db, dc;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          const float2 e = both(m.e[r][c_lane + c]), d = both(st.d[c]), x = both(st.du[c]);
+          const float2 e = both(o.e.v[c]), d = both(o.d.v[c]), x = both(o.d.v[c] * to_f(o.u.v[c]));
           float2 g2 = make_float2(0.f, 0.f), w2 = make_float2(0.f, 0.f);
 #pragma unroll
           for (int s = 0; s < S / 2; ++s) {
-            const float2 ex = decay(d, a2[c].v[s]);
             const float2 before = r == 0 ? h0[c].v[s] : h[r > 0 ? r - 1 : 0][c].v[s];
             const float2 g = fma2(Cn.v[s], e, carry[c].v[s]);
-            carry[c].v[s] = mul2(ex, g);
+            carry[c].v[s] = mul2(decay(d, a2[c].v[s]), g);
             const float2 w = mul2(carry[c].v[s], before);
-            w2 = fma2(w, a2[c].v[s], w2);
+            w2 = s == 0 ? mul2(w, a2[c].v[s]) : fma2(w, a2[c].v[s], w2);
             dA[c].v[s] = fma2(w, d, dA[c].v[s]);
-            g2 = fma2(g, Bn.v[s], g2);
+            g2 = s == 0 ? mul2(g, Bn.v[s]) : fma2(g, Bn.v[s], g2);
             db.v[s] = c == 0 ? mul2(g, x) : fma2(g, x, db.v[s]);
             dc.v[s] = c == 0 ? mul2(h[r][c].v[s], e) : fma2(h[r][c].v[s], e, dc.v[s]);
           }
@@ -266,8 +295,8 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
         reduce_scatter<2 * CH * UG, GS, 1>(v, lane);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          const int id = sg * NG + i, r = r0 + q * UG + id / (2 * CH), k = id % (2 * CH);
-          (k % 2 ? m.sum_w : m.sum_g)[r][c_lane + k / 2] = v[i];
+          const int id = sg * NG + i, r = r0 + q * UG + id / (2 * CH), j = id % (2 * CH);
+          (j % 2 ? m.sum_w : m.sum_g)[r][c_lane + j / 2] = v[i];
         }
       }
 #pragma unroll
@@ -278,60 +307,70 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
         reduce_scatter<2 * S * UB, LC, GS>(v, lane);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const int id = lane / GS * NB + i, r = r0 + q * UB + id / (2 * S), k = id % (2 * S);
-          m.bc[warp][r][k / S * NP + sg * S + k % S] = v[i];
+          const int id = lane / GS * NB + i, r = r0 + q * UB + id / (2 * S), j = id % (2 * S);
+          m.part[warp][r][j / S * NP + sg * S + j % S] = v[i];
         }
       }
     }
     __syncthreads();
 
+    {
+      float2 x[TURNS], y[TURNS], g[TURNS], slope[TURNS];
 #pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int r = Share::row(i);
-      const int64_t t = t0 + r;
-      if (t >= stop) continue;
-      const Chunk<T, V> cu = m.raw[slot][0][i][threadIdx.x], cd = m.raw[slot][1][i][threadIdx.x],
-                        cz = m.raw[slot][2][i][threadIdx.x], cy = m.raw[slot][3][i][threadIdx.x];
-      Chunk<T, V> ou, od, oz;
-      float slope[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) slope[j] = to_f(cd.v[j]) + bias[j];
-      if (a.softplus) by_two<V>(slope, sigmoid, sigmoid2);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float uf = to_f(cu.v[j]);
-        const float e = m.e[r][col + j], d = m.step[r][(col + j) / CH].d[(col + j) % CH], gB = m.sum_g[r][col + j];
-        float dd = fmaf(m.sum_w[r][col + j], kLn2, gB * uf);
-        if (a.softplus) dd *= slope[j];
-        if (t >= live) dd = 0.f;
-        ou.v[j] = from_f<T>(fmaf(d, gB, skip[j] * e));
-        od.v[j] = from_f<T>(dd);
-        dD[j] = fmaf(e, uf, dD[j]);
-        dbias[j] += dd;
+      for (int i = 0; i < TURNS; ++i) {
+        const int r = row0 + i * ROWS;
+        x[i] = load_pair(&act[0][r][col]);
+        g[i] = *reinterpret_cast<const float2*>(&m.sum_g[r][col]);
+        slope[i] = both(1.f);
       }
-      store_chunk<T, V>(du + t * a.channels, ou, left - col, a.vec);
-      store_chunk<T, V>(ddl + t * a.channels, od, left - col, a.vec);
+      if (a.softplus) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) slope[i] = sigmoid2(add2(load_pair(&act[1][row0 + i * ROWS][col]), bias));
+      }
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const int r = row0 + i * ROWS;
+        const int64_t t = t0 + r;
+        const float2 w = *reinterpret_cast<const float2*>(&m.sum_w[r][col]);
+        const float2 e = *reinterpret_cast<const float2*>(&m.e[r][col]);
+        const float2 d = *reinterpret_cast<const float2*>(&m.d[r][col]);
+        const float2 dd = r < rows ? mul2(slope[i], fma2(w, both(kLn2), mul2(g[i], x[i]))) : both(0.f);
+        dD = fma2(e, x[i], dD);
+        dbias = make_float2(dbias.x + dd.x, dbias.y + dd.y);
+        if (t < stop) {
+          store_chunk<T, 2>(du + t * a.channels, to_pair<T>(fma2(d, g[i], mul2(skip, e))), left - col, a.vec);
+          store_chunk<T, 2>(ddl + t * a.channels, to_pair<T>(dd), left - col, a.vec);
+        }
+      }
       if (a.z) {
-        float s[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = to_f(cz.v[j]);
-        by_two<V>(s, sigmoid, sigmoid2);
+        for (int i = 0; i < TURNS; ++i) {
+          const int r = row0 + i * ROWS;
+          const float2 z = load_pair(&act[3][r][col]), s = sigmoid2(z);
+          y[i] = fma2(skip, x[i], *reinterpret_cast<const float2*>(&m.sum_y[r][col]));
+          const float2 q = mul2(s, fma2(z, make_float2(1.f - s.x, 1.f - s.y), both(1.f)));
+          y[i] = r < rows ? mul2(mul2(load_pair(&act[2][r][col]), y[i]), q) : both(0.f);
+        }
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          oz.v[j] = from_f<T>(to_f(cy.v[j]) * fmaf(skip[j], to_f(cu.v[j]), m.sum_y[r][col + j]) *
-                              (s[j] * fmaf(to_f(cz.v[j]), 1.f - s[j], 1.f)));
-        store_chunk<T, V>(dz + t * a.channels, oz, left - col, a.vec);
+        for (int i = 0; i < TURNS; ++i) {
+          const int64_t t = t0 + row0 + i * ROWS;
+          if (t < stop) store_chunk<T, 2>(dz + t * a.channels, to_pair<T>(y[i]), left - col, a.vec);
+        }
       }
     }
-    for (int k = threadIdx.x; k < kScanTile * 2 * NP; k += NT) {
-      const int r = k / (2 * NP), n = k % (2 * NP);
+    for (int j = threadIdx.x; j < kScanTile * 2 * NP; j += NT) {
+      const int r = j / (2 * NP), n = j % (2 * NP);
       float v = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) v += m.bc[i][r][n];
-      if (t0 + r < live) part[(t0 + r) * 2 * NP + n] = v;
+      for (int i = 0; i < W; ++i) v += m.part[i][r][n];
+      if (r < rows) part[(t0 + r) * 2 * NP + n] = v;
     }
     __syncthreads();
+    if (slot) ++turn;
+    slot ^= 1;
   }
+  if (TILES && failed)  // copies that are late may not outlive the block
+    for (int i = 0; i < 2; ++i) mbar_wait_bounded(&m.bar[i], unsigned(turn) & 1u);
 
   if (a.dinit && at.seg == 0) {
 #pragma unroll
@@ -348,16 +387,21 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a)
 #pragma unroll
   for (int c = 0; c < CH; ++c)
     if (c_lane + c < left) *reinterpret_cast<Pairs<S>*>(a.part_a + (prow + c_lane + c) * NP + sg * S) = dA[c];
-  float* buf = &m.sum_y[0][0];  // sum_y, sum_g and sum_w: 48 CT floats for NT V = 16 CT / CNT
-  column_sums<Sh, V, Share::PER_ROW>(dD, buf);
-  column_sums<Sh, V, Share::PER_ROW>(dbias, buf);
-  if (threadIdx.x < Share::PER_ROW)
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (col + j < left) {
-        a.part_d[(prow + col + j) * 2] = dD[j];
-        a.part_d[(prow + col + j) * 2 + 1] = dbias[j];
-      }
+  float4* buf = reinterpret_cast<float4*>(&m.d[0][0]);  // d, e and the sums hold 80 CT floats, this takes 4 NT
+  static_assert(4 * NT <= 80 * CT, "room for the column sums");
+  __syncthreads();
+  buf[threadIdx.x] = make_float4(dD.x, dD.y, dbias.x, dbias.y);
+  __syncthreads();
+  if (threadIdx.x < PAIRS) {
+    float4 s = buf[threadIdx.x];
+    for (int r = 1; r < ROWS; ++r) {
+      const float4 v = buf[threadIdx.x + r * PAIRS];
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    float* p = a.part_d + (prow + col) * 2;
+    if (in0) p[0] = s.x, p[1] = s.z;
+    if (in1) p[2] = s.y, p[3] = s.w;
+  }
 }
 
 // dB, dC: sums of the channel tiles' partials, zero behind each sequence's end.
@@ -375,7 +419,16 @@ __global__ void __launch_bounds__(256) scan_bc_kernel(const ScanArgs a, int np) 
   float v = 0.f;
   if (t < scan_length(a, b)) {
     const float* p = a.part_bc + ((b * a.groups + g) * a.col_tiles * a.length + t) * 2 * np + n2;
-    for (int k = 0; k < a.col_tiles; ++k) v += p[int64_t(k) * a.length * 2 * np];
+    const int64_t step = a.length * 2 * np;
+    int k = 0;
+    for (; k + 16 <= a.col_tiles; k += 16) {  // loads in flight together, added in order
+      float x[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = p[(k + j) * step];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v += x[j];
+    }
+    for (; k < a.col_tiles; ++k) v += p[k * step];
   }
   T* out = static_cast<T*>(n2 < np ? a.dB : a.dC);
   out[((b * a.length + t) * a.groups + g) * a.states + n] = from_f<T>(v);
@@ -406,7 +459,7 @@ template <class F>
 static auto with_backward_shape(int64_t states, F&& f) {
   switch (scan_pad(states)) {
     case 4: return f(ScanShape<2, 2, 2, 2>{});
-    case 8: return f(ScanShape<4, 2, 2, 2>{});
+    case 8: return f(ScanShape<2, 2, 4, 4>{});
     case 16: return f(ScanShape<4, 2, 4, 4>{});
     case 32: return f(ScanShape<4, 2, 8, 4>{});
     default: return f(ScanShape<4, 2, 16, 4>{});
@@ -430,16 +483,19 @@ static BackwardLayout backward_layout(const bst_scan_desc* d, int segments) {
 int64_t scan_backward_workspace(const bst_scan_desc* d) { return backward_layout(d, 1).total; }
 
 template <typename T, class Sh>
-static int scan_backward_launch(ScanArgs a, cudaStream_t st) {
+static int scan_backward_launch(const bst_scan_desc* d, ScanArgs a, cudaStream_t st) {
   a.col_tiles = (a.per_group + Sh::CT - 1) / Sh::CT;
   const int64_t blocks = int64_t(a.batch) * a.segments * a.groups * a.col_tiles;
   const int64_t outs = int64_t(a.batch) * a.length * a.groups * 2 * Sh::NP;
   if (blocks > INT_MAX || outs / 256 + 1 > INT_MAX)
     return fail(BST_ERR_UNSUPPORTED, "the scan's gradients need more than 2^31 blocks");
   constexpr int smem = int(sizeof(BackwardShared<T, Sh>));
-  auto* kernel = scan_backward_kernel<T, Sh>;
+  ScanMaps maps;
+  if (a.mode == kCopyTiles && !scan_maps(d, Sh::CT, Sh::NP, a.u, a.delta, a.z, a.dy, a.B, a.C, &maps))
+    a.mode = kCopyWords;
+  auto* kernel = a.mode == kCopyTiles ? scan_backward_kernel<T, Sh, true> : scan_backward_kernel<T, Sh, false>;
   BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<unsigned(blocks), Sh::NT, smem, st>>>(a);
+  kernel<<<unsigned(blocks), Sh::NT, smem, st>>>(a, maps);
   if (int rc = launched("scan_backward_kernel launch")) return rc;
   scan_bc_kernel<T><<<unsigned((outs + 255) / 256), 256, 0, st>>>(a, Sh::NP);
   return launched("scan_bc_kernel launch");
@@ -486,14 +542,12 @@ extern "C" int bst_scan_backward(const bst_scan_desc* d, const void* u, const vo
   a.vec = aligned16(u) && aligned16(delta) && aligned16(z) && aligned16(dy) && aligned16(du) && aligned16(ddelta) &&
           aligned16(dz) &&
           (a.per_group | a.ub | a.us | a.db | a.ds | (z ? a.zb | a.zs : 0) | a.dyb | a.dys) % per == 0;
-  const uint64_t es = uint64_t(layer_elem_size(d->dtype));
-  auto at = [](const void* p) { return uint64_t(reinterpret_cast<uintptr_t>(p)); };
-  a.mode_act = copy_mode(at(u) | at(delta) | at(z) | at(dy) |
-                         es * (a.per_group | a.ub | a.us | a.db | a.ds | (z ? a.zb | a.zs : 0) | a.dyb | a.dys));
-  a.mode_bc = copy_mode((at(B) | at(C) | es * (a.states | a.Bb | a.Bs | a.Bg | a.Cb | a.Cs | a.Cg)) % 4 ? 1 : 4);
+  a.mode = scan_copy_mode(d, u, delta, z, dy, B, C);
+  a.error = device_error_word();
+  if (!a.error) return fail(BST_ERR_CUDA, "device error word unavailable");
   int rc = with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
-    return with_backward_shape(d->states, [&](auto sh) { return scan_backward_launch<T, decltype(sh)>(a, st); });
+    return with_backward_shape(d->states, [&](auto sh) { return scan_backward_launch<T, decltype(sh)>(d, a, st); });
   });
   if (rc) return rc;
   const int np = scan_pad(d->states);
