@@ -46,163 +46,190 @@ __device__ __forceinline__ float silu_slope(float p) {
   return s * fmaf(p, 1.f - s, 1.f);
 }
 
-// The W - 1 inputs before position t (t >= 0) of V channels: earlier positions of x, or the initial state.
+// The input at position t >= -(W - 1) of V channels: of x, or of the initial state.
 template <typename T, int V, int W>
-__device__ __forceinline__ Chunk<T, V> input_before(const ConvArgs& a, int64_t b, int64_t t, int c, int n) {
-  if (t >= 0) return load_chunk<T, V>(static_cast<const T*>(a.x) + b * a.xb + t * a.xs + c, n, a.vec);
-  Chunk<T, V> z;
-#pragma unroll
-  for (int i = 0; i < V; ++i) z.v[i] = from_f<T>(0.f);
-  if (!a.init) return z;
-  return load_chunk<T, V>(static_cast<const T*>(a.init) + (b * (W - 1) + t + W - 1) * a.channels + c, n, a.vec);
+__device__ __forceinline__ Chunk<T, V> input_at(const ConvArgs& a, int64_t b, int64_t t, int c) {
+  if (t >= 0) return load_whole<T, V>(static_cast<const T*>(a.x) + b * a.xb + t * a.xs + c, true);
+  return load_whole<T, V>(static_cast<const T*>(a.init) + (b * (W - 1) + t + W - 1) * a.channels + c, a.init != nullptr);
 }
 
-// grid: (channel vectors / threads, pieces, batch)
+// V channels as pairs (a pair of one where V is 1).
+template <int V>
+struct Lanes {
+  static constexpr int P = (V + 1) / 2;
+  float2 v[P];
+};
+template <typename T, int V>
+__device__ __forceinline__ Lanes<V> lanes(const Chunk<T, V>& c) {
+  Lanes<V> r;
+#pragma unroll
+  for (int i = 0; i < Lanes<V>::P; ++i)
+    r.v[i] = make_float2(to_f(c.v[2 * i]), V == 1 ? 0.f : to_f(c.v[V == 1 ? 0 : 2 * i + 1]));
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ Chunk<T, V> chunk(const Lanes<V>& l) {
+  Chunk<T, V> c;
+#pragma unroll
+  for (int i = 0; i < V; ++i) c.v[i] = from_f<T>(i % 2 ? l.v[i / 2].y : l.v[i / 2].x);
+  return c;
+}
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(128) conv_march_kernel(const ConvArgs a) {
-  const int c = (blockIdx.x * 128 + threadIdx.x) * V, n = a.channels - c;
-  if (n <= 0) return;
+__device__ __forceinline__ void load_weights(const ConvArgs& a, int c, Lanes<V> (&w)[W], Lanes<V>& bias) {
+#pragma unroll
+  for (int i = 0; i < 2 * Lanes<V>::P; ++i) {
+    const bool on = i < V;
+    (i % 2 ? bias.v[i / 2].y : bias.v[i / 2].x) = on && a.b ? conv_param<T>(a.b, a.wide, c + i) : 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+      (i % 2 ? w[k].v[i / 2].y : w[k].v[i / 2].x) = on ? conv_param<T>(a.w, a.wide, int64_t(c + i) * W + k) : 0.f;
+  }
+}
+
+constexpr int kMarchThreads = 128;
+
+// grid: (channel vectors / threads, pieces, batch).  V divides the channels.
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(kMarchThreads) conv_march_kernel(const ConvArgs a) {
+  constexpr int P = Lanes<V>::P;
+  const int c = (blockIdx.x * kMarchThreads + threadIdx.x) * V;
+  if (c >= a.channels) return;
   const int64_t b = blockIdx.z;
   const int64_t len = live_length(a.lengths, a.length, b);
-  const int64_t t0 = int64_t(blockIdx.y) * a.piece, t1 = min(t0 + a.piece, a.length);
-  float w[W][V], bias[V], win[W][V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = a.b && i < n ? conv_param<T>(a.b, a.wide, c + i) : 0.f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) w[k][i] = i < n ? conv_param<T>(a.w, a.wide, int64_t(c + i) * W + k) : 0.f;
-  }
-#pragma unroll
-  for (int k = 0; k < W - 1; ++k) {
-    Chunk<T, V> v{};
-    if (t0 < len) v = input_before<T, V, W>(a, b, t0 - (W - 1) + k, c, n);
-#pragma unroll
-    for (int i = 0; i < V; ++i) win[k][i] = to_f(v.v[i]);
-  }
+  const int64_t t0 = int64_t(blockIdx.y) * a.piece, t1 = min(t0 + a.piece, a.length), live = min(len, t1);
   const T* x = static_cast<const T*>(a.x) + b * a.xb + c;
   T* y = static_cast<T*>(a.y) + b * a.yb + c;
-  constexpr int U = 4;  // loads in flight per thread
-  for (int64_t t = t0; t < t1; t += U) {
-    Chunk<T, V> v[U];
+  constexpr int U = 4;  // positions per turn; those of the next turn are on their way meanwhile
+  Chunk<T, V> next[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load_chunk<T, V>(x + (t + u) * a.xs, t + u < min(len, t1) ? n : 0, a.vec);
+  for (int u = 0; u < U; ++u) next[u] = load_whole<T, V>(x + (t0 + u) * a.xs, t0 + u < live);
+  Lanes<V> w[W], bias, win[W - 1 + U];
+  load_weights<T, V, W>(a, c, w, bias);
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k)
+    win[k] = lanes<T, V>(t0 < len ? input_at<T, V, W>(a, b, t0 - (W - 1) + k, c) : Chunk<T, V>{});
+  for (int64_t t = t0; t < t1; t += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) win[W - 1 + u] = lanes<T, V>(next[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = load_whole<T, V>(x + (t + U + u) * a.xs, t + U + u < live);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      Chunk<T, V> o;
+      Lanes<V> p = bias;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        win[W - 1][i] = to_f(v[u].v[i]);
-        float p = bias[i];
+      for (int i = 0; i < P; ++i) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) p = fmaf(w[k][i], win[k][i], p);
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) win[k][i] = win[k + 1][i];
-        o.v[i] = from_f<T>(t + u < len ? (a.silu ? p * sigmoid(p) : p) : 0.f);
+        for (int k = 0; k < W; ++k) p.v[i] = fma2(w[k].v[i], win[u + k].v[i], p.v[i]);
+        if (a.silu) p.v[i] = mul2(p.v[i], sigmoid2(p.v[i]));
+        if (t + u >= len) p.v[i] = both(0.f);
       }
-      if (t + u < t1) store_chunk<T, V>(y + (t + u) * a.ys, o, n, a.vec);
+      store_whole<T, V>(y + (t + u) * a.ys, chunk<T, V>(p), t + u < t1);
     }
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) win[k] = win[U + k];
   }
   if (a.final_state && blockIdx.y == 0) {
     T* f = static_cast<T*>(a.final_state) + b * (W - 1) * a.channels + c;
 #pragma unroll
     for (int k = 0; k < W - 1; ++k)
-      store_chunk<T, V>(f + int64_t(k) * a.channels, input_before<T, V, W>(a, b, len - (W - 1) + k, c, n), n, a.vec);
+      store_whole<T, V>(f + int64_t(k) * a.channels, input_at<T, V, W>(a, b, len - (W - 1) + k, c), true);
   }
 }
 
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(128) conv_march_backward_kernel(const ConvArgs a) {
-  const int c = (blockIdx.x * 128 + threadIdx.x) * V, n = a.channels - c;
-  if (n <= 0) return;
+__global__ void __launch_bounds__(kMarchThreads) conv_march_backward_kernel(const ConvArgs a) {
+  constexpr int P = Lanes<V>::P;
+  const int c = (blockIdx.x * kMarchThreads + threadIdx.x) * V;
+  if (c >= a.channels) return;
   const int64_t b = blockIdx.z;
   const int64_t len = live_length(a.lengths, a.length, b);
   const int64_t t0 = int64_t(blockIdx.y) * a.piece, t1 = min(t0 + a.piece, a.length);
-  float w[W][V], bias[V], xw[W][V], qw[W][V], dw[W][V], db[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = a.b && i < n ? conv_param<T>(a.b, a.wide, c + i) : 0.f;
-    db[i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      w[k][i] = i < n ? conv_param<T>(a.w, a.wide, int64_t(c + i) * W + k) : 0.f;
-      qw[k][i] = dw[k][i] = 0.f;
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < W - 1; ++k) {
-    Chunk<T, V> v{};
-    if (t0 < len) v = input_before<T, V, W>(a, b, t0 - (W - 1) + k, c, n);
-#pragma unroll
-    for (int i = 0; i < V; ++i) xw[k][i] = to_f(v.v[i]);
-  }
+  const int64_t last = min(len, t1 + W - 1);  // positions that this piece reads
   const T* x = static_cast<const T*>(a.x) + b * a.xb + c;
   const T* dy = static_cast<const T*>(a.dy) + b * a.dyb + c;
   T* dx = static_cast<T*>(a.dx) + b * a.dxb + c;
   const T* df = a.dfinal ? static_cast<const T*>(a.dfinal) + b * (W - 1) * a.channels + c : nullptr;
-  constexpr int U = 2;
+  constexpr int U = 4;
+  Chunk<T, V> nx[U], nd[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    nx[u] = load_whole<T, V>(x + (t0 + u) * a.xs, t0 + u < last);
+    nd[u] = load_whole<T, V>(dy + (t0 + u) * a.dys, t0 + u < last);
+  }
+  Lanes<V> w[W], bias, xw[W - 1 + U], qw[W - 1 + U], dw[W], db;
+  load_weights<T, V, W>(a, c, w, bias);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    db.v[i] = both(0.f);
+#pragma unroll
+    for (int k = 0; k < W; ++k) dw[k].v[i] = both(0.f);
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) qw[k].v[i] = both(0.f);
+  }
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k)
+    xw[k] = lanes<T, V>(t0 < len ? input_at<T, V, W>(a, b, t0 - (W - 1) + k, c) : Chunk<T, V>{});
   // Step j brings q[j] in and completes dx[j - W + 1]; q is zero from `len` on.
   for (int64_t j0 = t0; j0 < t1 + W - 1; j0 += U) {
-    Chunk<T, V> vx[U], vd[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int m = j0 + u < len && j0 + u < t1 + W - 1 ? n : 0;
-      vx[u] = load_chunk<T, V>(x + (j0 + u) * a.xs, m, a.vec);
-      vd[u] = load_chunk<T, V>(dy + (j0 + u) * a.dys, m, a.vec);
+      xw[W - 1 + u] = lanes<T, V>(nx[u]);
+      qw[W - 1 + u] = lanes<T, V>(nd[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      nx[u] = load_whole<T, V>(x + (j0 + U + u) * a.xs, j0 + U + u < last);
+      nd[u] = load_whole<T, V>(dy + (j0 + U + u) * a.dys, j0 + U + u < last);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t j = j0 + u, t = j - (W - 1);
-      const bool own = j < t1;  // q[j] counts towards dw here, not in the next piece
-      float g[V];
+      Lanes<V> g;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        xw[W - 1][i] = to_f(vx[u].v[i]);
-        float q = to_f(vd[u].v[i]);
+      for (int i = 0; i < P; ++i) {
+        float2 q = qw[W - 1 + u].v[i];
         if (a.silu) {
-          float p = bias[i];
+          float2 p = bias.v[i];
 #pragma unroll
-          for (int k = 0; k < W; ++k) p = fmaf(w[k][i], xw[k][i], p);
-          q = j < len ? q * silu_slope(p) : 0.f;
+          for (int k = 0; k < W; ++k) p = fma2(w[k].v[i], xw[u + k].v[i], p);
+          const float2 s = sigmoid2(p);
+          q = mul2(q, mul2(s, fma2(p, make_float2(1.f - s.x, 1.f - s.y), both(1.f))));
+          if (j >= last) q = both(0.f);
+          qw[W - 1 + u].v[i] = q;
         }
-        qw[W - 1][i] = q;
-        const float qo = own ? q : 0.f;
-        db[i] += qo;
-        g[i] = 0.f;
+        const float2 own = j < t1 ? q : both(0.f);  // the others count towards dw in the next piece
+        db.v[i] = add2(db.v[i], own);
+        g.v[i] = both(0.f);
 #pragma unroll
         for (int k = 0; k < W; ++k) {
-          dw[k][i] = fmaf(qo, xw[k][i], dw[k][i]);
-          g[i] = fmaf(w[k][i], qw[W - 1 - k][i], g[i]);
-        }
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) {
-          xw[k][i] = xw[k + 1][i];
-          qw[k][i] = qw[k + 1][i];
+          dw[k].v[i] = fma2(own, xw[u + k].v[i], dw[k].v[i]);
+          g.v[i] = fma2(w[k].v[i], qw[W - 1 + u - k].v[i], g.v[i]);
         }
       }
-      if (j >= t1 + W - 1) continue;
       // The first piece also completes the gradients of the W - 1 inputs before position 0.
-      if (t < t0 && !(t0 == 0 && a.dinit)) continue;
-      if (df && t < len && t >= len - (W - 1)) {
-        const Chunk<T, V> f = load_chunk<T, V>(df + (t - (len - (W - 1))) * a.channels, n, a.vec);
+      const bool edge = t < 0 && a.dinit && j < t1 + W - 1;
+      if (df && t < len && t >= len - (W - 1) && (t >= t0 || edge)) {
+        const Lanes<V> f = lanes<T, V>(load_whole<T, V>(df + (t - (len - (W - 1))) * a.channels, true));
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] += to_f(f.v[i]);
+        for (int i = 0; i < P; ++i) g.v[i] = add2(g.v[i], f.v[i]);
       }
-      Chunk<T, V> o;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o.v[i] = from_f<T>(t < len ? g[i] : 0.f);
-      if (t >= 0) store_chunk<T, V>(dx + t * a.dxs, o, n, a.vec);
-      else
-        store_chunk<T, V>(static_cast<T*>(a.dinit) + (b * (W - 1) + t + W - 1) * a.channels + c, o, n, a.vec);
+      for (int i = 0; i < P; ++i)
+        if (t >= len) g.v[i] = both(0.f);
+      store_whole<T, V>(dx + t * a.dxs, chunk<T, V>(g), t >= t0 && t < t1);
+      if (edge)
+        store_whole<T, V>(static_cast<T*>(a.dinit) + (b * (W - 1) + t + W - 1) * a.channels + c, chunk<T, V>(g), true);
+    }
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+      xw[k] = xw[U + k];
+      qw[k] = qw[U + k];
     }
   }
   float* part = a.part + (b * a.pieces + blockIdx.y) * (W + 1) * a.channels + c;
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (i < n) {
-#pragma unroll
-      for (int k = 0; k < W; ++k) part[int64_t(k) * a.channels + i] = dw[k][i];
-      part[int64_t(W) * a.channels + i] = db[i];
-    }
+  for (int k = 0; k <= W; ++k)
+    store_whole<float, V>(part + int64_t(k) * a.channels, chunk<float, V>(k < W ? dw[k < W ? k : 0] : db), true);
 }
 
 // ---- sequence contiguous ---------------------------------------------------------------
@@ -331,38 +358,35 @@ __global__ void __launch_bounds__(1024) conv_params_kernel(const float* part, in
 // out_state may be the state itself.
 template <typename T, int V>
 __global__ void __launch_bounds__(128) conv_step_kernel(const ConvArgs a, int width, int64_t state_b, int64_t out_b) {
-  const int per = (a.channels + V - 1) / V;
+  const int per = a.channels / V;  // V divides the channels
   const int64_t i = int64_t(blockIdx.x) * 128 + threadIdx.x;
   const int64_t b = i / per;
   if (b >= a.length) return;  // `length` holds the batch here
-  const int c = int(i % per) * V, n = a.channels - c;
+  const int c = int(i % per) * V;
   const T* state = static_cast<const T*>(a.init) + b * state_b + c;
   T* out = static_cast<T*>(a.final_state) + b * out_b + c;
   Chunk<T, V> rows[8];
 #pragma unroll
   for (int k = 0; k < 7; ++k)
-    if (k < width - 1) rows[k] = load_chunk<T, V>(state + int64_t(k) * a.channels, n, a.vec);
-  const Chunk<T, V> x = load_chunk<T, V>(static_cast<const T*>(a.x) + b * a.xb + c, n, a.vec);
+    if (k < width - 1) rows[k] = load_whole<T, V>(state + int64_t(k) * a.channels, true);
+  const Chunk<T, V> x = load_whole<T, V>(static_cast<const T*>(a.x) + b * a.xb + c, true);
   float p[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    p[j] = 0.f;
-    if (j < n) {
-      p[j] = a.b ? conv_param<T>(a.b, a.wide, c + j) : 0.f;
+    p[j] = a.b ? conv_param<T>(a.b, a.wide, c + j) : 0.f;
 #pragma unroll
-      for (int k = 0; k < 7; ++k)
-        if (k < width - 1) p[j] = fmaf(conv_param<T>(a.w, a.wide, int64_t(c + j) * width + k), to_f(rows[k].v[j]), p[j]);
-      p[j] = fmaf(conv_param<T>(a.w, a.wide, int64_t(c + j) * width + width - 1), to_f(x.v[j]), p[j]);
-    }
+    for (int k = 0; k < 7; ++k)
+      if (k < width - 1) p[j] = fmaf(conv_param<T>(a.w, a.wide, int64_t(c + j) * width + k), to_f(rows[k].v[j]), p[j]);
+    p[j] = fmaf(conv_param<T>(a.w, a.wide, int64_t(c + j) * width + width - 1), to_f(x.v[j]), p[j]);
   }
   Chunk<T, V> o;
 #pragma unroll
   for (int j = 0; j < V; ++j) o.v[j] = from_f<T>(a.silu ? p[j] * sigmoid(p[j]) : p[j]);
-  store_chunk<T, V>(static_cast<T*>(a.y) + b * a.yb + c, o, n, a.vec);
+  store_whole<T, V>(static_cast<T*>(a.y) + b * a.yb + c, o, true);
 #pragma unroll
   for (int k = 1; k < 7; ++k)
-    if (k < width - 1) store_chunk<T, V>(out + int64_t(k - 1) * a.channels, rows[k], n, a.vec);
-  if (width > 1) store_chunk<T, V>(out + int64_t(width - 2) * a.channels, x, n, a.vec);
+    if (k < width - 1) store_whole<T, V>(out + int64_t(k - 1) * a.channels, rows[k], true);
+  if (width > 1) store_whole<T, V>(out + int64_t(width - 2) * a.channels, x, true);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -418,11 +442,11 @@ static int with_width(int width, F&& f) {
   }
 }
 
-// Channels per thread of the marching kernels: a 16-byte vector where everything is aligned to it and
-// the window fits the registers (W <= 4), else single channels.
-template <typename T, class F>
+// Channels per thread of the marching kernels: a vector where everything is aligned to 16 bytes and the window fits
+// the registers (W <= 4), else single channels.  The backward pass keeps three times the forward's numbers per
+// channel and takes 4 channels (8 bytes in 16-bit types), the forward pass 16 bytes.
+template <typename T, int VW, class F>
 static int with_vector(const ConvArgs& a, int width, F&& f) {
-  constexpr int VW = 16 / int(sizeof(T));
   if (a.vec && width <= 4) return f(std::integral_constant<int, VW>{});
   return f(std::integral_constant<int, 1>{});
 }
@@ -455,7 +479,7 @@ int bst_causal_conv_forward(const bst_conv_desc* d, const void* x, const void* w
         conv_lines_kernel<T, W><<<dim3(unsigned(d->channels), pieces, unsigned(d->batch)), 256, 0, st>>>(a);
         return launched("conv_lines_kernel launch");
       }
-      return with_vector<T>(a, W, [&](auto v) {
+      return with_vector<T, 16 / int(sizeof(T))>(a, W, [&](auto v) {
         constexpr int V = W <= 4 ? decltype(v)::value : 1;
         const unsigned cols = unsigned((d->channels + 128 * V - 1) / (128 * V));
         conv_march_kernel<T, V, W><<<dim3(cols, pieces, unsigned(d->batch)), 128, 0, st>>>(a);
@@ -509,7 +533,7 @@ int bst_causal_conv_backward(const bst_conv_desc* d, const void* x, const void* 
         conv_lines_backward_kernel<T, W><<<lines, 256, 0, st>>>(a);
         return launched("conv_lines_backward_kernel launch");
       }
-      return with_vector<T>(a, W, [&](auto v) {
+      return with_vector<T, 4>(a, W, [&](auto v) {
         constexpr int V = W <= 4 ? decltype(v)::value : 1;
         const unsigned cols = unsigned((d->channels + 128 * V - 1) / (128 * V));
         conv_march_backward_kernel<T, V, W>

@@ -60,6 +60,19 @@ __device__ __forceinline__ void store_chunk(T* p, const Chunk<T, V>& c, int n, b
   }
 }
 
+// All V elements or none (zeros): one predicated access, so that the loads of a loop's next turn can stay in flight
+// (a choice between paths, as above, makes the thread wait for the values where the paths meet).
+template <typename T, int V>
+__device__ __forceinline__ Chunk<T, V> load_whole(const T* p, bool on) {
+  Chunk<T, V> c{};
+  if (on) c = *reinterpret_cast<const Chunk<T, V>*>(p);
+  return c;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_whole(T* p, const Chunk<T, V>& c, bool on) {
+  if (on) *reinterpret_cast<Chunk<T, V>*>(p) = c;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -35,6 +35,29 @@ template <typename T>
 __device__ __forceinline__ float param_at(const void* p, int wide, int i) {
   return wide ? static_cast<const float*>(p)[i] : to_f(static_cast<const T*>(p)[i]);
 }
+// Parameters i .. i + V - 1 (`missing` where there are none).
+template <typename T, int V>
+__device__ __forceinline__ void load_params(const void* p, int wide, int i, int dim, float missing,
+                                            float (&v)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = missing;
+  } else if (V > 1 && i < dim) {  // more than one column per access: dim is a multiple of V, all is aligned
+    if (wide) {
+      const Chunk<float, V < 4 ? V : 4>* q = reinterpret_cast<const Chunk<float, V < 4 ? V : 4>*>(
+          static_cast<const float*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = q[j / 4].v[j % 4];
+    } else {
+      const Chunk<T, V> c = *reinterpret_cast<const Chunk<T, V>*>(static_cast<const T*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = to_f(c.v[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = i + j < dim ? param_at<T>(p, wide, i + j) : missing;
+  }
+}
 
 // Sum of v over the TPR threads of a row's slot, known to all of them.  `buf`: TPR / 32 floats of the slot.
 template <int TPR>
@@ -60,40 +83,49 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2* buf) {
 template <int TPR, int V>
 __device__ __forceinline__ int column(int t, int k) { return (k * TPR + t) * V; }
 
+// The parameters of a thread's columns and the next row are on their way, or here, while a row is worked on.
 template <typename T, int TPR, int V>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_forward_kernel(const NormArgs a) {
   constexpr int NT = TPR < 256 ? 256 : TPR, SLOTS = NT / TPR, NC = kNormItems / V;
   __shared__ float2 buf[SLOTS][TPR / 32];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-  // Every slot of the block makes the same number of turns: the sums hold barriers.
-  for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += int64_t(gridDim.x) * SLOTS) {
-    const int64_t row = row0 + slot;
-    const bool live = row < a.rows;
-    const T* x = static_cast<const T*>(a.x) + row * a.xs;
-    Chunk<T, V> c[NC];
+  const int64_t stride = int64_t(gridDim.x) * SLOTS;
+  int64_t row = int64_t(blockIdx.x) * SLOTS + slot;
+  Chunk<T, V> c[NC];
+  auto load = [&](int64_t r) {
+    const T* x = static_cast<const T*>(a.x) + r * a.xs;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int i = column<TPR, V>(t, k);
-      c[k] = load_chunk<T, V>(x + i, live ? a.dim - i : 0, a.vec);
+      c[k] = load_whole<T, V>(x + i, r < a.rows && i < a.dim);
     }
-    float s = 0.f;
+  };
+  load(row);
+  float w[NC][V], b[NC][V];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    load_params<T, V>(a.w, a.wide, column<TPR, V>(t, k), a.dim, 1.f, w[k]);
+    load_params<T, V>(a.b, a.wide, column<TPR, V>(t, k), a.dim, 0.f, b[k]);
+  }
+  // Every slot of the block makes the same number of turns: the sums hold barriers.
+  for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += stride, row += stride) {
+    float x[NC][V], s = 0.f, q = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) s += to_f(c[k].v[j]);
+      for (int j = 0; j < V; ++j) s += x[k][j] = to_f(c[k].v[j]);
+    load(row + stride);
     const float mean = row_sum2<TPR>(make_float2(s, 0.f), buf[slot]).x * a.inv_dim;
-    float q = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (column<TPR, V>(t, k) + j < a.dim) {
-          const float d = to_f(c[k].v[j]) - mean;
-          q = fmaf(d, d, q);
-        }
+      for (int j = 0; j < V; ++j) {
+        x[k][j] = column<TPR, V>(t, k) + j < a.dim ? x[k][j] - mean : 0.f;
+        q = fmaf(x[k][j], x[k][j], q);
+      }
     const float var = row_sum2<TPR>(make_float2(q, 0.f), buf[slot]).x * a.inv_dim;
     const float rstd = 1.f / sqrtf(var + a.eps);
-    if (!live) continue;
+    if (row >= a.rows) continue;
     if (t == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -101,18 +133,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_forward_kernel(con
     T* y = static_cast<T*>(a.y) + row * a.ys;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const int i = column<TPR, V>(t, k);
-      if (i < a.dim) {
-        Chunk<T, V> o;
+      Chunk<T, V> o;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (i + j < a.dim) {
-            const float w = a.w ? param_at<T>(a.w, a.wide, i + j) : 1.f;
-            const float b = a.b ? param_at<T>(a.b, a.wide, i + j) : 0.f;
-            o.v[j] = from_f<T>(fmaf((to_f(c[k].v[j]) - mean) * rstd, w, b));
-          }
-        store_chunk<T, V>(y + i, o, a.dim - i, a.vec);
-      }
+      for (int j = 0; j < V; ++j) o.v[j] = from_f<T>(fmaf(x[k][j] * rstd, w[k][j], b[k][j]));
+      const int i = column<TPR, V>(t, k);
+      store_whole<T, V>(y + i, o, i < a.dim);
     }
   }
 }
@@ -122,45 +147,54 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
   constexpr int NT = TPR < 256 ? 256 : TPR, SLOTS = NT / TPR, NC = kNormItems / V;
   __shared__ float2 buf[SLOTS][TPR / 32];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-  float w[kNormItems], dw[kNormItems], db[kNormItems];
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int i = column<TPR, V>(t, k) + j;
-      w[k * V + j] = a.w && i < a.dim ? param_at<T>(a.w, a.wide, i) : 1.f;
-      dw[k * V + j] = db[k * V + j] = 0.f;
-    }
-  for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += int64_t(gridDim.x) * SLOTS) {
-    const int64_t row = row0 + slot;
-    const bool live = row < a.rows;
-    const T* x = static_cast<const T*>(a.x) + row * a.xs;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.dys;
-    Chunk<T, V> cx[NC], cd[NC];
+  const int64_t stride = int64_t(gridDim.x) * SLOTS;
+  int64_t row = int64_t(blockIdx.x) * SLOTS + slot;
+  Chunk<T, V> nx[NC], nd[NC];
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto load = [&](int64_t r) {
+    const bool live = r < a.rows;
+    const T* x = static_cast<const T*>(a.x) + r * a.xs;
+    const T* dy = static_cast<const T*>(a.dy) + r * a.dys;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int i = column<TPR, V>(t, k);
-      cx[k] = load_chunk<T, V>(x + i, live ? a.dim - i : 0, a.vec);
-      cd[k] = load_chunk<T, V>(dy + i, live ? a.dim - i : 0, a.vec);
+      nx[k] = load_whole<T, V>(x + i, live && i < a.dim);
+      nd[k] = load_whole<T, V>(dy + i, live && i < a.dim);
     }
-    const float mean = live ? a.mean_in[row] : 0.f, rstd = live ? a.rstd_in[row] : 0.f;
+    next_mean = live ? a.mean_in[r] : 0.f;
+    next_rstd = live ? a.rstd_in[r] : 0.f;
+  };
+  load(row);
+  float w[NC][V], dw[NC][V], db[NC][V];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    load_params<T, V>(a.w, a.wide, column<TPR, V>(t, k), a.dim, 1.f, w[k]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.f;
+  }
+  for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += stride, row += stride) {
+    Chunk<T, V> cx[NC], cd[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) cx[k] = nx[k], cd[k] = nd[k];
+    const float mean = next_mean, rstd = next_rstd;
+    if (row0 + stride < a.rows) load(row + stride);
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        // Columns beyond dim hold dy = 0, so that only their xh has to be kept out of nothing.
+        // Columns beyond dim hold dy = 0.
         const float d = to_f(cd[k].v[j]);
         const float xh = (to_f(cx[k].v[j]) - mean) * rstd;
-        const float g = d * w[k * V + j];
+        const float g = d * w[k][j];
         s.x += g;
         s.y = fmaf(g, xh, s.y);
-        dw[k * V + j] = fmaf(d, xh, dw[k * V + j]);
-        db[k * V + j] += d;
+        dw[k][j] = fmaf(d, xh, dw[k][j]);
+        db[k][j] += d;
       }
     s = row_sum2<TPR>(s, buf[slot]);
     const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
-    if (!live) continue;
+    if (row >= a.rows) continue;
     T* dx = static_cast<T*>(a.dx) + row * a.dxs;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
@@ -169,9 +203,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float xh = (to_f(cx[k].v[j]) - mean) * rstd;
-        o.v[j] = from_f<T>(rstd * (to_f(cd[k].v[j]) * w[k * V + j] - m1 - xh * m2));
+        o.v[j] = from_f<T>(rstd * (to_f(cd[k].v[j]) * w[k][j] - m1 - xh * m2));
       }
-      store_chunk<T, V>(dx + i, o, a.dim - i, a.vec);
+      store_whole<T, V>(dx + i, o, i < a.dim);
     }
   }
   if (!a.params) return;
@@ -182,8 +216,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
     for (int j = 0; j < V; ++j) {
       const int i = column<TPR, V>(t, k) + j;
       if (i < a.dim) {
-        p[i] = dw[k * V + j];
-        p[a.dim + i] = db[k * V + j];
+        p[i] = dw[k][j];
+        p[a.dim + i] = db[k][j];
       }
     }
 }
@@ -343,12 +377,15 @@ int bst_layer_norm_forward(const bst_norm_desc* d, const void* x, const void* we
   a.x = x, a.w = weight, a.b = bias, a.y = y, a.mean = mean, a.rstd = rstd;
   a.rows = d->rows, a.xs = d->x_row, a.ys = d->y_row, a.dim = int(d->dim);
   a.wide = d->param_dtype == BST_F32 && d->dtype != BST_F32;
-  a.vec = aligned16(x) && aligned16(y) && d->dim % per == 0 && d->x_row % per == 0 && d->y_row % per == 0;
+  a.vec = aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias) && d->dim % per == 0 && d->x_row % per == 0 && d->y_row % per == 0;
   a.eps = float(d->eps), a.inv_dim = 1.f / float(d->dim);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int tpr = norm_threads(d->dim);
   const int slots = tpr && tpr < 256 ? 256 / tpr : 1;
-  const unsigned blocks = unsigned(std::min<int64_t>((d->rows + slots - 1) / slots, INT_MAX));
+  // Blocks that walk over the rows keep their parameters: as many as are resident (1024 threads per SM), long rows
+  // one block each.
+  const int64_t resident = tpr ? int64_t(sm_count()) * 1024 / std::max(tpr, 256) : INT_MAX;
+  const unsigned blocks = unsigned(std::min<int64_t>((d->rows + slots - 1) / slots, resident));
   return with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
     if (tpr) return norm_launch<T, false>(a, tpr, blocks, st);
@@ -387,7 +424,7 @@ int bst_layer_norm_backward(const bst_norm_desc* d, const void* x, const void* w
   a.part = static_cast<float*>(workspace);
   a.rows = d->rows, a.xs = d->x_row, a.dys = d->dy_row, a.dxs = d->dx_row, a.dim = int(d->dim);
   a.wide = d->param_dtype == BST_F32 && d->dtype != BST_F32;
-  a.vec = aligned16(x) && aligned16(dy) && aligned16(dx) && d->dim % per == 0 && d->x_row % per == 0 &&
+  a.vec = aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(weight) && d->dim % per == 0 && d->x_row % per == 0 &&
           d->dy_row % per == 0 && d->dx_row % per == 0;
   a.params = params;
   a.inv_dim = 1.f / float(d->dim);

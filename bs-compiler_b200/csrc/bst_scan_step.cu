@@ -17,7 +17,7 @@ struct StepArgs {
   void* y;
   float* out;
   int64_t ub, db, zb, yb, Bb, Bg, Cb, Cg, sb, sc, ob, oc;
-  int64_t rows;  // batch * channels
+  int64_t batch;
   int channels, per_group, states, softplus;
 };
 
@@ -28,47 +28,64 @@ __device__ __forceinline__ void load_floats(const T* p, float (&v)[V]) {
   for (int i = 0; i < V; ++i) v[i] = to_f(c.v[i]);
 }
 
-// L lanes per channel, V states per access (states % V == 0).
-template <typename T, int L, int V>
+// L lanes per channel, V states per access (states % V == 0), K = ceil(states / (L V)) accesses per lane, NB sequences
+// per thread: what belongs to the channel (A, D, the step's bias) is read once for them, and their states are on
+// their way together.
+template <typename T, int L, int V, int K, int NB>
 __global__ void __launch_bounds__(256) scan_step_kernel(const StepArgs a) {
-  const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / L;
-  const int l = threadIdx.x % L;
-  const bool on = row < a.rows;
-  const int64_t b = on ? row / a.channels : 0;
-  const int c = on ? int(row % a.channels) : 0, g = c / a.per_group;
-  const float raw = to_f(static_cast<const T*>(a.delta)[b * a.db + c]) + (a.dbias ? a.dbias[c] : 0.f);
-  const float u = to_f(static_cast<const T*>(a.u)[b * a.ub + c]);
-  const float d = a.softplus ? softplus(raw) : raw;
-  const float du = d * u, d2 = d * kLog2e;
-  const float* A = a.A + int64_t(c) * a.states;
-  const float* h = a.state + b * a.sb + c * a.sc;
-  float* out = a.out + b * a.ob + c * a.oc;
-  const T* B = static_cast<const T*>(a.B) + b * a.Bb + g * a.Bg;
-  const T* C = static_cast<const T*>(a.C) + b * a.Cb + g * a.Cg;
-  float y = 0.f;
-  for (int n = l * V; n < a.states; n += L * V) {
-    float hv[V], Av[V], Bv[V], Cv[V];
-    load_floats<float, V>(h + n, hv);
-    load_floats<float, V>(A + n, Av);
-    load_floats<T, V>(B + n, Bv);
-    load_floats<T, V>(C + n, Cv);
-    Chunk<float, V> o;
+  const int i = int(blockIdx.x) * (256 / L) + int(threadIdx.x) / L, l = threadIdx.x % L;
+  const bool in = i < a.channels;
+  const int c = in ? i : 0, g = c / a.per_group;
+  const int64_t b0 = int64_t(blockIdx.y) * NB;
+  float hv[NB][K][V], Av[K][V], raw[NB], u[NB], z[NB];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      o.v[i] = fmaf(ex2(d2 * Av[i]), hv[i], du * Bv[i]);
-      y = fmaf(o.v[i], Cv[i], y);
-    }
-    if (on) *reinterpret_cast<Chunk<float, V>*>(out + n) = o;
+  for (int k = 0; k < K; ++k) {
+    const int n = (k * L + l) * V;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (n < a.states && b0 + j < a.batch) load_floats<float, V>(a.state + (b0 + j) * a.sb + c * a.sc + n, hv[j][k]);
+    if (n < a.states) load_floats<float, V>(a.A + int64_t(c) * a.states + n, Av[k]);
+  }
+  const float bias = a.dbias ? a.dbias[c] : 0.f, skip = a.D ? a.D[c] : 0.f;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int64_t b = b0 + j < a.batch ? b0 + j : 0;
+    raw[j] = to_f(static_cast<const T*>(a.delta)[b * a.db + c]);
+    u[j] = to_f(static_cast<const T*>(a.u)[b * a.ub + c]);
+    z[j] = a.z ? to_f(static_cast<const T*>(a.z)[b * a.zb + c]) : 0.f;
   }
 #pragma unroll
-  for (int m = L / 2; m >= 1; m >>= 1) y += __shfl_xor_sync(0xffffffffu, y, m);
-  if (on && l == 0) {
-    if (a.D) y = fmaf(a.D[c], u, y);
-    if (a.z) {
-      const float z = to_f(static_cast<const T*>(a.z)[b * a.zb + c]);
-      y *= z * sigmoid(z);
+  for (int j = 0; j < NB; ++j) {
+    if (b0 + j >= a.batch) break;
+    const int64_t b = b0 + j;
+    const float d = a.softplus ? softplus(raw[j] + bias) : raw[j] + bias;
+    const float du = d * u[j], d2 = d * kLog2e;
+    const T* B = static_cast<const T*>(a.B) + b * a.Bb + g * a.Bg;
+    const T* C = static_cast<const T*>(a.C) + b * a.Cb + g * a.Cg;
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int n = (k * L + l) * V;
+      if (n < a.states) {
+        float Bv[V], Cv[V];
+        load_floats<T, V>(B + n, Bv);
+        load_floats<T, V>(C + n, Cv);
+        Chunk<float, V> o;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          o.v[v] = fmaf(ex2(d2 * Av[k][v]), hv[j][k][v], du * Bv[v]);
+          y = fmaf(o.v[v], Cv[v], y);
+        }
+        if (in) *reinterpret_cast<Chunk<float, V>*>(a.out + b * a.ob + c * a.oc + n) = o;
+      }
     }
-    static_cast<T*>(a.y)[b * a.yb + c] = from_f<T>(y);
+#pragma unroll
+    for (int m = L / 2; m >= 1; m >>= 1) y += __shfl_xor_sync(0xffffffffu, y, m);
+    if (in && l == 0) {
+      y = fmaf(skip, u[j], y);
+      if (a.z) y *= z[j] * sigmoid(z[j]);
+      static_cast<T*>(a.y)[b * a.yb + c] = from_f<T>(y);
+    }
   }
 }
 
@@ -90,24 +107,37 @@ extern "C" int bst_scan_step(const bst_scan_desc* d, const void* u, const void* 
   a.ub = d->u_batch, a.db = d->delta_batch, a.zb = d->z_batch, a.yb = d->y_batch;
   a.Bb = d->B_batch, a.Bg = d->B_group, a.Cb = d->C_batch, a.Cg = d->C_group;
   a.sb = state_batch, a.sc = state_channel, a.ob = out_batch, a.oc = out_channel;
-  a.rows = d->batch * d->channels, a.channels = int(d->channels), a.per_group = int(d->channels / d->groups);
+  a.batch = d->batch, a.channels = int(d->channels), a.per_group = int(d->channels / d->groups);
   a.states = int(d->states), a.softplus = d->softplus != 0;
   const bool vec = aligned16(A) && aligned16(B) && aligned16(C) && aligned16(state) && aligned16(out_state) &&
                    (d->states | a.Bb | a.Bg | a.Cb | a.Cg | a.sb | a.sc | a.ob | a.oc) % 4 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
-    auto go = [&](auto lc, auto vc) {
-      constexpr int L = decltype(lc)::value, V = decltype(vc)::value;
-      const int64_t blocks = (a.rows * L + 255) / 256;
-      if (blocks > INT_MAX) return fail(BST_ERR_UNSUPPORTED, "the step needs more than 2^31 blocks");
-      scan_step_kernel<T, L, V><<<unsigned(blocks), 256, 0, st>>>(a);
-      return launched("scan_step_kernel launch");
-    };
     using std::integral_constant;
-    if (!vec) return go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    if (d->states <= 8) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-    if (d->states <= 16) return go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-    return go(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    // Four sequences per thread where that leaves two full turns of blocks (256 x 4096 x 16: 57 us with one, 25 with
+    // four), one where threads are scarce.
+    auto go = [&](auto lc, auto vc, auto kc) {
+      constexpr int L = decltype(lc)::value, V = decltype(vc)::value, K = decltype(kc)::value;
+      const int64_t cols = (d->channels * L + 255) / 256;
+      auto launch = [&](auto nb) {
+        constexpr int NB = decltype(nb)::value;
+        const int64_t turns = (d->batch + NB - 1) / NB;
+        if (turns > 65535) return fail(BST_ERR_UNSUPPORTED, "the step takes up to 65535 sequences (more in large batches)");
+        scan_step_kernel<T, L, V, K, NB><<<dim3(unsigned(cols), unsigned(turns)), 256, 0, st>>>(a);
+        return launched("scan_step_kernel launch");
+      };
+      if (K <= 2 && cols * ((d->batch + 3) / 4) >= int64_t(sm_count()) * 16) return launch(integral_constant<int, 4>{});
+      return launch(integral_constant<int, 1>{});
+    };
+    integral_constant<int, 1> one;
+    integral_constant<int, 2> two;
+    integral_constant<int, 4> four;
+    integral_constant<int, 8> eight;
+    if (!vec) return go(eight, one, eight);
+    if (d->states <= 8) return go(two, four, one);
+    if (d->states <= 16) return go(four, four, one);
+    if (d->states <= 32) return go(eight, four, one);
+    return go(eight, four, two);
   });
 }
