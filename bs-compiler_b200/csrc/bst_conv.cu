@@ -74,23 +74,43 @@ __device__ __forceinline__ Chunk<T, V> chunk(const Lanes<V>& l) {
   for (int i = 0; i < V; ++i) c.v[i] = from_f<T>(i % 2 ? l.v[i / 2].y : l.v[i / 2].x);
   return c;
 }
+template <int V>
+__device__ __forceinline__ void set_lane(Lanes<V>& l, int i, float v) { (i % 2 ? l.v[i / 2].y : l.v[i / 2].x) = v; }
+// The weights of V channels are V W neighbouring elements.
+template <typename P, int V, int W>
+__device__ __forceinline__ void load_weights_as(const P* w, const P* b, int c, Lanes<V> (&out)[W], Lanes<V>& bias) {
+  constexpr int Q = V % 4 == 0 ? 4 : V % 2 == 0 ? 2 : 1;
+#pragma unroll
+  for (int q = 0; q < V * W / Q; ++q) {
+    const Chunk<P, Q> k = load_whole<P, Q>(w + int64_t(c) * W + q * Q, true);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) set_lane<V>(out[(q * Q + i) % W], (q * Q + i) / W, to_f(k.v[i]));
+  }
+#pragma unroll
+  for (int q = 0; q < V / Q; ++q) {
+    const Chunk<P, Q> k = load_whole<P, Q>(b + c + q * Q, b != nullptr);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) set_lane<V>(bias, q * Q + i, to_f(k.v[i]));
+  }
+  if (V == 1) {  // the pair's other half
+    bias.v[0].y = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) out[k].v[0].y = 0.f;
+  }
+}
 template <typename T, int V, int W>
 __device__ __forceinline__ void load_weights(const ConvArgs& a, int c, Lanes<V> (&w)[W], Lanes<V>& bias) {
-#pragma unroll
-  for (int i = 0; i < 2 * Lanes<V>::P; ++i) {
-    const bool on = i < V;
-    (i % 2 ? bias.v[i / 2].y : bias.v[i / 2].x) = on && a.b ? conv_param<T>(a.b, a.wide, c + i) : 0.f;
-#pragma unroll
-    for (int k = 0; k < W; ++k)
-      (i % 2 ? w[k].v[i / 2].y : w[k].v[i / 2].x) = on ? conv_param<T>(a.w, a.wide, int64_t(c + i) * W + k) : 0.f;
-  }
+  if (a.wide)
+    load_weights_as<float, V, W>(static_cast<const float*>(a.w), static_cast<const float*>(a.b), c, w, bias);
+  else
+    load_weights_as<T, V, W>(static_cast<const T*>(a.w), static_cast<const T*>(a.b), c, w, bias);
 }
 
 constexpr int kMarchThreads = 128;
 
 // grid: (channel vectors / threads, pieces, batch).  V divides the channels.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kMarchThreads) conv_march_kernel(const ConvArgs a) {
+__global__ void __launch_bounds__(kMarchThreads, 6) conv_march_kernel(const ConvArgs a) {
   constexpr int P = Lanes<V>::P;
   const int c = (blockIdx.x * kMarchThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
@@ -108,7 +128,9 @@ __global__ void __launch_bounds__(kMarchThreads) conv_march_kernel(const ConvArg
 #pragma unroll
   for (int k = 0; k < W - 1; ++k)
     win[k] = lanes<T, V>(t0 < len ? input_at<T, V, W>(a, b, t0 - (W - 1) + k, c) : Chunk<T, V>{});
-  for (int64_t t = t0; t < t1; t += U) {
+  // `whole`: no position of the turn lies behind the sequence or the piece.
+  auto turn = [&](auto whole, int64_t t) {
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
     for (int u = 0; u < U; ++u) win[W - 1 + u] = lanes<T, V>(next[u]);
 #pragma unroll
@@ -121,12 +143,16 @@ __global__ void __launch_bounds__(kMarchThreads) conv_march_kernel(const ConvArg
 #pragma unroll
         for (int k = 0; k < W; ++k) p.v[i] = fma2(w[k].v[i], win[u + k].v[i], p.v[i]);
         if (a.silu) p.v[i] = mul2(p.v[i], sigmoid2(p.v[i]));
-        if (t + u >= len) p.v[i] = both(0.f);
+        if (!WHOLE && t + u >= len) p.v[i] = both(0.f);
       }
-      store_whole<T, V>(y + (t + u) * a.ys, chunk<T, V>(p), t + u < t1);
+      store_whole<T, V>(y + (t + u) * a.ys, chunk<T, V>(p), WHOLE || t + u < t1);
     }
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) win[k] = win[U + k];
+  };
+  for (int64_t t = t0; t < t1; t += U) {
+    if (t + U <= live) turn(std::true_type{}, t);
+    else turn(std::false_type{}, t);
   }
   if (a.final_state && blockIdx.y == 0) {
     T* f = static_cast<T*>(a.final_state) + b * (W - 1) * a.channels + c;
@@ -137,7 +163,7 @@ __global__ void __launch_bounds__(kMarchThreads) conv_march_kernel(const ConvArg
 }
 
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kMarchThreads) conv_march_backward_kernel(const ConvArgs a) {
+__global__ void __launch_bounds__(kMarchThreads, 3) conv_march_backward_kernel(const ConvArgs a) {
   constexpr int P = Lanes<V>::P;
   const int c = (blockIdx.x * kMarchThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
@@ -169,8 +195,10 @@ __global__ void __launch_bounds__(kMarchThreads) conv_march_backward_kernel(cons
 #pragma unroll
   for (int k = 0; k < W - 1; ++k)
     xw[k] = lanes<T, V>(t0 < len ? input_at<T, V, W>(a, b, t0 - (W - 1) + k, c) : Chunk<T, V>{});
-  // Step j brings q[j] in and completes dx[j - W + 1]; q is zero from `len` on.
-  for (int64_t j0 = t0; j0 < t1 + W - 1; j0 += U) {
+  // Step j brings q[j] in and completes dx[j - W + 1]; q is zero from `len` on.  `whole`: all positions of the turn
+  // belong to this piece and none to an edge of the sequence.
+  auto turn = [&](auto whole, int64_t j0) {
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       xw[W - 1 + u] = lanes<T, V>(nx[u]);
@@ -194,37 +222,46 @@ __global__ void __launch_bounds__(kMarchThreads) conv_march_backward_kernel(cons
           for (int k = 0; k < W; ++k) p = fma2(w[k].v[i], xw[u + k].v[i], p);
           const float2 s = sigmoid2(p);
           q = mul2(q, mul2(s, fma2(p, make_float2(1.f - s.x, 1.f - s.y), both(1.f))));
-          if (j >= last) q = both(0.f);
+          if (!WHOLE && j >= last) q = both(0.f);
           qw[W - 1 + u].v[i] = q;
         }
-        const float2 own = j < t1 ? q : both(0.f);  // the others count towards dw in the next piece
+        const float2 own = WHOLE || j < t1 ? q : both(0.f);  // the others count towards dw in the next piece
         db.v[i] = add2(db.v[i], own);
-        g.v[i] = both(0.f);
 #pragma unroll
         for (int k = 0; k < W; ++k) {
           dw[k].v[i] = fma2(own, xw[u + k].v[i], dw[k].v[i]);
-          g.v[i] = fma2(w[k].v[i], qw[W - 1 + u - k].v[i], g.v[i]);
+          g.v[i] = k == 0 ? mul2(w[k].v[i], qw[W - 1 + u].v[i]) : fma2(w[k].v[i], qw[W - 1 + u - k].v[i], g.v[i]);
         }
       }
-      // The first piece also completes the gradients of the W - 1 inputs before position 0.
-      const bool edge = t < 0 && a.dinit && j < t1 + W - 1;
-      if (df && t < len && t >= len - (W - 1) && (t >= t0 || edge)) {
-        const Lanes<V> f = lanes<T, V>(load_whole<T, V>(df + (t - (len - (W - 1))) * a.channels, true));
+      if constexpr (WHOLE) {
+        store_whole<T, V>(dx + t * a.dxs, chunk<T, V>(g), true);
+      } else {
+        // The first piece also completes the gradients of the W - 1 inputs before position 0.
+        const bool edge = t < 0 && a.dinit && j < t1 + W - 1;
+        if (df && t < len && t >= len - (W - 1) && (t >= t0 || edge)) {
+          const Lanes<V> f = lanes<T, V>(load_whole<T, V>(df + (t - (len - (W - 1))) * a.channels, true));
 #pragma unroll
-        for (int i = 0; i < P; ++i) g.v[i] = add2(g.v[i], f.v[i]);
+          for (int i = 0; i < P; ++i) g.v[i] = add2(g.v[i], f.v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+          if (t >= len) g.v[i] = both(0.f);
+        store_whole<T, V>(dx + t * a.dxs, chunk<T, V>(g), t >= t0 && t < t1);
+        if (edge)
+          store_whole<T, V>(static_cast<T*>(a.dinit) + (b * (W - 1) + t + W - 1) * a.channels + c, chunk<T, V>(g),
+                            true);
       }
-#pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (t >= len) g.v[i] = both(0.f);
-      store_whole<T, V>(dx + t * a.dxs, chunk<T, V>(g), t >= t0 && t < t1);
-      if (edge)
-        store_whole<T, V>(static_cast<T*>(a.dinit) + (b * (W - 1) + t + W - 1) * a.channels + c, chunk<T, V>(g), true);
     }
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
       xw[k] = xw[U + k];
       qw[k] = qw[U + k];
     }
+  };
+  for (int64_t j0 = t0; j0 < t1 + W - 1; j0 += U) {
+    // dx[t] of the turn: t0 <= t, and none of the last W - 1 positions, which the final state's gradient may join
+    if (j0 >= t0 + W - 1 && j0 + U <= t1 && j0 + U <= len) turn(std::true_type{}, j0);
+    else turn(std::false_type{}, j0);
   }
   float* part = a.part + (b * a.pieces + blockIdx.y) * (W + 1) * a.channels + c;
 #pragma unroll
@@ -340,8 +377,17 @@ __global__ void __launch_bounds__(1024) conv_params_kernel(const float* part, in
   const int c = threadIdx.x % 32, r = threadIdx.x / 32;
   const int64_t n = int64_t(width + 1) * channels, i = int64_t(blockIdx.x) * 32 + c;
   float s = 0.f;
-  if (i < n)
-    for (int64_t k = r; k < rows; k += 32) s += part[k * n + i];
+  if (i < n) {
+    int64_t k = r;
+    for (; k + 7 * 32 < rows; k += 8 * 32) {  // loads in flight together, added in order
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = part[(k + j * 32) * n + i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; k < rows; k += 32) s += part[k * n + i];
+  }
   sums[r][c] = s;
   __syncthreads();
   s = warp_sum(sums[c][r]);
@@ -408,12 +454,11 @@ static int conv_check(const bst_conv_desc* d) {
 static int conv_piece(const bst_conv_desc* d, bool backward) {
   const int64_t least = (d->length + 65534) / 65535;  // the grid's limit on pieces
   if (d->lines) return int(std::max<int64_t>(1024, least));
-  const int64_t per = 16 / layer_elem_size(d->dtype);
-  const int64_t threads = std::max<int64_t>(1, d->batch * ((d->channels + per - 1) / per));
-  const int64_t want = int64_t(sm_count()) * (backward ? 512 : 1024);
+  const int64_t threads = std::max<int64_t>(1, d->batch * ((d->channels + 3) / 4));
+  const int64_t want = int64_t(sm_count()) * (backward ? 1536 : 2048);
   const int64_t pieces = std::max<int64_t>(1, (want + threads - 1) / threads);
   int64_t piece = (d->length + pieces - 1) / pieces;
-  piece = std::max<int64_t>(16, (piece + 3) / 4 * 4);
+  piece = std::max<int64_t>(16, (piece + 7) / 8 * 8);
   return int(std::max(piece, least));
 }
 
@@ -443,9 +488,9 @@ static int with_width(int width, F&& f) {
 }
 
 // Channels per thread of the marching kernels: a vector where everything is aligned to 16 bytes and the window fits
-// the registers (W <= 4), else single channels.  The backward pass keeps three times the forward's numbers per
-// channel and takes 4 channels (8 bytes in 16-bit types), the forward pass 16 bytes.
-template <typename T, int VW, class F>
+// the registers (W <= 4), else single channels.  Four channels (8 bytes in 16-bit types): eight halve the warps that
+// fit, and with them the bytes under way (1 x 8192 x 4096 in bf16: 53 us with eight).
+template <int VW, class F>
 static int with_vector(const ConvArgs& a, int width, F&& f) {
   if (a.vec && width <= 4) return f(std::integral_constant<int, VW>{});
   return f(std::integral_constant<int, 1>{});
@@ -468,6 +513,7 @@ int bst_causal_conv_forward(const bst_conv_desc* d, const void* x, const void* w
   a.x = x, a.w = weight, a.b = bias, a.init = initial, a.y = y, a.final_state = final_state, a.lengths = lengths;
   const int64_t per = 16 / layer_elem_size(d->dtype);
   a.vec = !d->lines && aligned16(x) && aligned16(y) && aligned16(initial) && aligned16(final_state) &&
+          aligned16(weight) && aligned16(bias) &&
           (d->channels | a.xb | a.xs | a.yb | a.ys) % per == 0;
   if (d->length == 0 && !final_state) return BST_OK;
   const unsigned pieces = unsigned(std::max(a.pieces, 1));  // no positions: one piece hands the state on
@@ -479,7 +525,7 @@ int bst_causal_conv_forward(const bst_conv_desc* d, const void* x, const void* w
         conv_lines_kernel<T, W><<<dim3(unsigned(d->channels), pieces, unsigned(d->batch)), 256, 0, st>>>(a);
         return launched("conv_lines_kernel launch");
       }
-      return with_vector<T, 16 / int(sizeof(T))>(a, W, [&](auto v) {
+      return with_vector<4>(a, W, [&](auto v) {
         constexpr int V = W <= 4 ? decltype(v)::value : 1;
         const unsigned cols = unsigned((d->channels + 128 * V - 1) / (128 * V));
         conv_march_kernel<T, V, W><<<dim3(cols, pieces, unsigned(d->batch)), 128, 0, st>>>(a);
@@ -523,6 +569,7 @@ int bst_causal_conv_backward(const bst_conv_desc* d, const void* x, const void* 
   a.x = x, a.w = weight, a.b = bias, a.init = initial, a.lengths = lengths, a.dy = dy, a.dfinal = dfinal;
   a.dx = dx, a.dinit = dinitial, a.part = static_cast<float*>(workspace);
   a.vec = !d->lines && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(initial) && aligned16(dfinal) &&
+          aligned16(weight) && aligned16(bias) &&
           aligned16(dinitial) && (d->channels | a.xb | a.xs | a.dyb | a.dys | a.dxb | a.dxs) % per == 0;
   int rc = with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
@@ -533,7 +580,7 @@ int bst_causal_conv_backward(const bst_conv_desc* d, const void* x, const void* 
         conv_lines_backward_kernel<T, W><<<lines, 256, 0, st>>>(a);
         return launched("conv_lines_backward_kernel launch");
       }
-      return with_vector<T, 4>(a, W, [&](auto v) {
+      return with_vector<4>(a, W, [&](auto v) {
         constexpr int V = W <= 4 ? decltype(v)::value : 1;
         const unsigned cols = unsigned((d->channels + 128 * V - 1) / (128 * V));
         conv_march_backward_kernel<T, V, W>

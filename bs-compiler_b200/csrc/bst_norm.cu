@@ -13,9 +13,12 @@
 // launch adds the partial rows up in a fixed order.
 #include <algorithm>
 
+#include "bst_kernels.cuh"  // mbarrier helpers
 #include "bst_layer.cuh"
 
 namespace bst {
+
+int occupancy(const void* fn, int threads, int smem);  // bst_core.cu
 
 constexpr int kNormItems = 16;        // elements of a row per thread
 constexpr int kNormMaxThreads = 1024; // longer rows than 1024 * 16 go through the kernels that re-read
@@ -29,6 +32,8 @@ struct NormArgs {
   int64_t rows, xs, ys, dys, dxs;
   int dim, wide, vec, params;     // wide: parameters are fp32; params: dw or db asked for
   float eps, inv_dim;
+  int stages;       // of the ring
+  unsigned* error;  // the device's error word
 };
 
 template <typename T>
@@ -59,48 +64,115 @@ __device__ __forceinline__ void load_params(const void* p, int wide, int i, int 
   }
 }
 
-// Sum of v over the TPR threads of a row's slot, known to all of them.  `buf`: TPR / 32 floats of the slot.
-template <int TPR>
-__device__ __forceinline__ float2 row_sum2(float2 v, float2* buf) {
-  v.x = warp_sum(v.x);
-  v.y = warp_sum(v.y);
+// Sums of v over the TPR threads of a row's slot, known to all of them.  `buf`: two halves of TPR / 32 entries for the
+// slot, used in turn (`half`), so that one barrier per sum is enough.
+template <int TPR, typename V>
+__device__ __forceinline__ V row_sum(V v, V (*buf)[TPR / 32], int& half) {
+  constexpr bool TWO = sizeof(V) == sizeof(float2);
+  auto lane_sum = [](V x, int m) {
+    if constexpr (TWO) {
+      x.x += __shfl_xor_sync(0xffffffffu, x.x, m);
+      x.y += __shfl_xor_sync(0xffffffffu, x.y, m);
+    } else {
+      x += __shfl_xor_sync(0xffffffffu, x, m);
+    }
+    return x;
+  };
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) v = lane_sum(v, m);
   if constexpr (TPR > 32) {
     const int t = threadIdx.x % TPR;
-    __syncthreads();  // the previous sum has been read
-    if (t % 32 == 0) buf[t / 32] = v;
+    V* to = buf[half];
+    half ^= 1;
+    if (t % 32 == 0) to[t / 32] = v;
     __syncthreads();
-    v = make_float2(0.f, 0.f);
+    v = to[t % (TPR / 32)];
 #pragma unroll
-    for (int i = 0; i < TPR / 32; ++i) {
-      v.x += buf[i].x;
-      v.y += buf[i].y;
-    }
+    for (int m = TPR / 64; m >= 1; m >>= 1) v = lane_sum(v, m);
   }
   return v;
 }
+
+// Rows on their way into shared memory: a ring of STAGES rows of each of N tensors per slot, filled by the bulk copy
+// engine (whole rows, 16-byte aligned).  It keeps more bytes under way than the threads' registers could.
+constexpr int kNormMaxStages = 4;
+constexpr int kNormRingHeader = 256;  // the barriers of up to 8 slots
+constexpr int kNormRingMost = 200 * 1024;  // two stages of a block's rows have to fit in shared memory
+template <typename T, int N>
+struct RowRing {
+  T* data;         // [stages][N][dim] of this slot
+  uint64_t* bar;   // [stages]
+  int dim, stages;
+  bool failed;
+
+  __device__ __forceinline__ void start(unsigned char* shared, int n, int slot, int d, bool leader) {
+    dim = d;
+    stages = n;
+    failed = false;
+    bar = reinterpret_cast<uint64_t*>(shared) + slot * kNormMaxStages;
+    data = reinterpret_cast<T*>(shared + kNormRingHeader) + int64_t(slot) * n * N * d;
+    if (leader) {
+      for (int i = 0; i < n; ++i) mbar_init(&bar[i], 1);
+      mbar_fence_init();
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ T* row(int stage, int n) const { return data + (stage * N + n) * int64_t(dim); }
+  __device__ __forceinline__ void expect(int stage) { mbar_expect_tx(&bar[stage], unsigned(N * dim * sizeof(T))); }
+  __device__ __forceinline__ void copy(int stage, int n, const T* from) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(row(stage, n))),
+                 "l"(from), "r"(unsigned(dim * sizeof(T))), "r"(smem_u32(&bar[stage]))
+                 : "memory");
+  }
+  __device__ __forceinline__ void wait(int stage, unsigned parity, unsigned* error) {
+    if (!failed && !mbar_wait_bounded(&bar[stage], parity)) {
+      failed = true;
+      atomicOr(error, kErrTmaTimeout);
+    }
+  }
+};
 
 // First column of chunk k of thread t of a row.
 template <int TPR, int V>
 __device__ __forceinline__ int column(int t, int k) { return (k * TPR + t) * V; }
 
-// The parameters of a thread's columns and the next row are on their way, or here, while a row is worked on.
+// The parameters of a thread's columns stay in its registers.  Rows arrive ahead of their turn: through the ring where
+// whole vectors can be read (V > 1), one row ahead in registers otherwise.
 template <typename T, int TPR, int V>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_forward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : 768 / (TPR < 256 ? 256 : TPR))
+    norm_forward_kernel(const NormArgs a) {
   constexpr int NT = TPR < 256 ? 256 : TPR, SLOTS = NT / TPR, NC = kNormItems / V;
-  __shared__ float2 buf[SLOTS][TPR / 32];
+  constexpr bool RING = V > 1;
+  __shared__ float buf[SLOTS][2][TPR / 32];
+  extern __shared__ __align__(128) unsigned char shared[];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  int half = 0, stage = 0;
+  unsigned parity = 0;
   const int64_t stride = int64_t(gridDim.x) * SLOTS;
   int64_t row = int64_t(blockIdx.x) * SLOTS + slot;
+  const T* base = static_cast<const T*>(a.x);
+  RowRing<T, 1> ring;
   Chunk<T, V> c[NC];
   auto load = [&](int64_t r) {
-    const T* x = static_cast<const T*>(a.x) + r * a.xs;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int i = column<TPR, V>(t, k);
-      c[k] = load_whole<T, V>(x + i, r < a.rows && i < a.dim);
+      c[k] = load_whole<T, V>(base + r * a.xs + i, r < a.rows && i < a.dim);
     }
   };
-  load(row);
+  auto send = [&](int to, int64_t r) {
+    if (t == 0 && r < a.rows) {
+      ring.expect(to);
+      ring.copy(to, 0, base + r * a.xs);
+    }
+  };
+  if constexpr (RING) {
+    ring.start(shared, a.stages, slot, a.dim, t == 0);
+    for (int i = 0; i < a.stages; ++i) send(i, row + i * stride);
+  } else {
+    load(row);
+  }
   float w[NC][V], b[NC][V];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
@@ -109,13 +181,26 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_forward_kernel(con
   }
   // Every slot of the block makes the same number of turns: the sums hold barriers.
   for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += stride, row += stride) {
+    if constexpr (RING) {
+      if (row < a.rows) ring.wait(stage, parity, a.error);
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const int i = column<TPR, V>(t, k);
+        c[k] = load_whole<T, V>(ring.row(stage, 0) + i, row < a.rows && i < a.dim);
+      }
+    }
     float x[NC][V], s = 0.f, q = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) s += x[k][j] = to_f(c[k].v[j]);
-    load(row + stride);
-    const float mean = row_sum2<TPR>(make_float2(s, 0.f), buf[slot]).x * a.inv_dim;
+    if constexpr (!RING) load(row + stride);
+    const float mean = row_sum<TPR>(s, buf[slot], half) * a.inv_dim;
+    if constexpr (RING) {  // everybody has read the row: its place is free
+      if (TPR == 32) __syncwarp();
+      send(stage, row + a.stages * stride);
+      if (++stage == a.stages) stage = 0, parity ^= 1;
+    }
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -123,7 +208,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_forward_kernel(con
         x[k][j] = column<TPR, V>(t, k) + j < a.dim ? x[k][j] - mean : 0.f;
         q = fmaf(x[k][j], x[k][j], q);
       }
-    const float var = row_sum2<TPR>(make_float2(q, 0.f), buf[slot]).x * a.inv_dim;
+    const float var = row_sum<TPR>(q, buf[slot], half) * a.inv_dim;
     const float rstd = 1.f / sqrtf(var + a.eps);
     if (row >= a.rows) continue;
     if (t == 0) {
@@ -140,15 +225,22 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_forward_kernel(con
       store_whole<T, V>(y + i, o, i < a.dim);
     }
   }
+  if (RING && ring.failed)  // a row that is late may not outlive the block
+    for (int i = 0; i < a.stages; ++i) mbar_wait_bounded(&ring.bar[i], parity);
 }
 
 template <typename T, int TPR, int V>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 256 ? 1 : 2) norm_backward_kernel(const NormArgs a) {
   constexpr int NT = TPR < 256 ? 256 : TPR, SLOTS = NT / TPR, NC = kNormItems / V;
-  __shared__ float2 buf[SLOTS][TPR / 32];
+  constexpr bool RING = V > 1;
+  __shared__ float2 buf[SLOTS][2][TPR / 32];
+  extern __shared__ __align__(128) unsigned char shared[];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  int half = 0, stage = 0;
+  unsigned parity = 0;
   const int64_t stride = int64_t(gridDim.x) * SLOTS;
   int64_t row = int64_t(blockIdx.x) * SLOTS + slot;
+  RowRing<T, 2> ring;
   Chunk<T, V> nx[NC], nd[NC];
   float next_mean = 0.f, next_rstd = 0.f;
   auto load = [&](int64_t r) {
@@ -164,7 +256,21 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
     next_mean = live ? a.mean_in[r] : 0.f;
     next_rstd = live ? a.rstd_in[r] : 0.f;
   };
-  load(row);
+  auto send = [&](int to, int64_t r) {
+    if (t == 0 && r < a.rows) {
+      ring.expect(to);
+      ring.copy(to, 0, static_cast<const T*>(a.x) + r * a.xs);
+      ring.copy(to, 1, static_cast<const T*>(a.dy) + r * a.dys);
+    }
+  };
+  if constexpr (RING) {
+    ring.start(shared, a.stages, slot, a.dim, t == 0);
+    for (int i = 0; i < a.stages; ++i) send(i, row + i * stride);
+    next_mean = row < a.rows ? a.mean_in[row] : 0.f;
+    next_rstd = row < a.rows ? a.rstd_in[row] : 0.f;
+  } else {
+    load(row);
+  }
   float w[NC][V], dw[NC][V], db[NC][V];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
@@ -174,10 +280,23 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
   }
   for (int64_t row0 = int64_t(blockIdx.x) * SLOTS; row0 < a.rows; row0 += stride, row += stride) {
     Chunk<T, V> cx[NC], cd[NC];
-#pragma unroll
-    for (int k = 0; k < NC; ++k) cx[k] = nx[k], cd[k] = nd[k];
     const float mean = next_mean, rstd = next_rstd;
-    if (row0 + stride < a.rows) load(row + stride);
+    if constexpr (RING) {
+      const bool live = row < a.rows, more = row + stride < a.rows;
+      if (live) ring.wait(stage, parity, a.error);
+      next_mean = more ? a.mean_in[row + stride] : 0.f;
+      next_rstd = more ? a.rstd_in[row + stride] : 0.f;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const int i = column<TPR, V>(t, k);
+        cx[k] = load_whole<T, V>(ring.row(stage, 0) + i, live && i < a.dim);
+        cd[k] = load_whole<T, V>(ring.row(stage, 1) + i, live && i < a.dim);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NC; ++k) cx[k] = nx[k], cd[k] = nd[k];
+      if (row0 + stride < a.rows) load(row + stride);
+    }
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -192,7 +311,12 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
         dw[k][j] = fmaf(d, xh, dw[k][j]);
         db[k][j] += d;
       }
-    s = row_sum2<TPR>(s, buf[slot]);
+    s = row_sum<TPR>(s, buf[slot], half);
+    if constexpr (RING) {  // everybody has read the row: its place is free
+      if (TPR == 32) __syncwarp();
+      send(stage, row + a.stages * stride);
+      if (++stage == a.stages) stage = 0, parity ^= 1;
+    }
     const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
     if (row >= a.rows) continue;
     T* dx = static_cast<T*>(a.dx) + row * a.dxs;
@@ -208,6 +332,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
       store_whole<T, V>(dx + i, o, i < a.dim);
     }
   }
+  if (RING && ring.failed)  // a row that is late may not outlive the block
+    for (int i = 0; i < a.stages; ++i) mbar_wait_bounded(&ring.bar[i], parity);
   if (!a.params) return;
   float* p = a.part + (int64_t(blockIdx.x) * SLOTS + slot) * 2 * a.dim;
 #pragma unroll
@@ -225,18 +351,19 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_backward_kernel(co
 // ---- rows too long for a block's registers: the row is read again for each sum ------------
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_forward_long_kernel(const NormArgs a) {
-  __shared__ float2 buf[32];
+  __shared__ float buf[2][32];
+  int half = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.xs;
     T* y = static_cast<T*>(a.y) + row * a.ys;
     float s = 0.f, q = 0.f;
     for (int i = threadIdx.x; i < a.dim; i += 1024) s += to_f(x[i]);
-    const float mean = row_sum2<1024>(make_float2(s, 0.f), buf).x * a.inv_dim;
+    const float mean = row_sum<1024>(s, buf, half) * a.inv_dim;
     for (int i = threadIdx.x; i < a.dim; i += 1024) {
       const float d = to_f(x[i]) - mean;
       q = fmaf(d, d, q);
     }
-    const float rstd = 1.f / sqrtf(row_sum2<1024>(make_float2(q, 0.f), buf).x * a.inv_dim + a.eps);
+    const float rstd = 1.f / sqrtf(row_sum<1024>(q, buf, half) * a.inv_dim + a.eps);
     if (threadIdx.x == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -250,7 +377,8 @@ __global__ void __launch_bounds__(1024) norm_forward_long_kernel(const NormArgs 
 
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_backward_long_kernel(const NormArgs a) {
-  __shared__ float2 buf[32];
+  __shared__ float2 buf[2][32];
+  int half = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.xs;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dys;
@@ -262,7 +390,7 @@ __global__ void __launch_bounds__(1024) norm_backward_long_kernel(const NormArgs
       s.x += g;
       s.y = fmaf(g, (to_f(x[i]) - mean) * rstd, s.y);
     }
-    s = row_sum2<1024>(s, buf);
+    s = row_sum<1024>(s, buf, half);
     const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
     for (int i = threadIdx.x; i < a.dim; i += 1024) {
       const float g = to_f(dy[i]) * (a.w ? param_at<T>(a.w, a.wide, i) : 1.f);
@@ -294,8 +422,17 @@ __global__ void __launch_bounds__(1024) norm_params_kernel(const float* part, in
   const int c = threadIdx.x % 32, r = threadIdx.x / 32;
   const int64_t i = int64_t(blockIdx.x) * 32 + c, n = 2 * int64_t(dim);
   float s = 0.f;
-  if (i < n)
-    for (int64_t k = r; k < slots; k += 32) s += part[k * n + i];
+  if (i < n) {
+    int64_t k = r;
+    for (; k + 7 * 32 < slots; k += 8 * 32) {  // loads in flight together, added in order
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = part[(k + j * 32) * n + i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; k < slots; k += 32) s += part[k * n + i];
+  }
   sums[r][c] = s;
   __syncthreads();
   s = warp_sum(sums[c][r]);  // warp r now adds up column r of the block
@@ -315,11 +452,11 @@ static int norm_threads(int64_t dim) {
     if (dim <= int64_t(t) * kNormItems) return t;
   return 0;
 }
-constexpr int kNormBlocksPerSm = 2;  // of the backward pass: each of its slots leaves a partial row
+constexpr int kNormBlocksPerSm = 2;  // of the backward pass (its launch bounds): each slot leaves a partial row
 
 static int64_t norm_backward_blocks(int64_t rows, int tpr) {
   const int slots = tpr < 256 ? 256 / tpr : 1;
-  return std::max<int64_t>(1, std::min<int64_t>((rows + slots - 1) / slots, int64_t(sm_count()) * kNormBlocksPerSm));
+  return std::max<int64_t>(1, std::min<int64_t>((rows + slots - 1) / slots, int64_t(sm_count()) * (tpr > 256 ? 1 : kNormBlocksPerSm)));
 }
 static int64_t norm_slots(const bst_norm_desc* d) {
   const int tpr = norm_threads(d->dim);
@@ -339,13 +476,26 @@ static int norm_check(const bst_norm_desc* d) {
 }
 
 template <typename T, bool BWD>
-static int norm_launch(const NormArgs& a, int tpr, unsigned blocks, cudaStream_t st) {
+static int norm_launch(const NormArgs& a, int tpr, int64_t blocks, cudaStream_t st) {
   constexpr int VW = 16 / int(sizeof(T));
   auto go = [&](auto tprc, auto vc) {
     constexpr int TPR = decltype(tprc)::value, V = decltype(vc)::value;
     constexpr int NT = TPR < 256 ? 256 : TPR;
-    if constexpr (BWD) norm_backward_kernel<T, TPR, V><<<blocks, NT, 0, st>>>(a);
-    else norm_forward_kernel<T, TPR, V><<<blocks, NT, 0, st>>>(a);
+    const int stage = (NT / TPR) * (BWD ? 2 : 1) * a.dim * int(sizeof(T));
+    NormArgs args = a;
+    args.stages = std::max(2, std::min(kNormMaxStages, 64 * 1024 / stage));
+    const int smem = V > 1 ? kNormRingHeader + args.stages * stage : 0;
+    if constexpr (BWD) {
+      auto* kernel = norm_backward_kernel<T, TPR, V>;
+      BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      kernel<<<unsigned(blocks), NT, smem, st>>>(args);
+    } else {
+      // A block walks over the rows and keeps its parameters: no more of them than are resident.
+      auto* kernel = norm_forward_kernel<T, TPR, V>;
+      BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      const int64_t most = int64_t(sm_count()) * std::max(1, occupancy((const void*)kernel, NT, smem));
+      kernel<<<unsigned(std::min(blocks, most)), NT, smem, st>>>(args);
+    }
     return launched(BWD ? "norm_backward_kernel launch" : "norm_forward_kernel launch");
   };
   auto pick = [&](auto tprc) {
@@ -379,17 +529,17 @@ int bst_layer_norm_forward(const bst_norm_desc* d, const void* x, const void* we
   a.wide = d->param_dtype == BST_F32 && d->dtype != BST_F32;
   a.vec = aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias) && d->dim % per == 0 && d->x_row % per == 0 && d->y_row % per == 0;
   a.eps = float(d->eps), a.inv_dim = 1.f / float(d->dim);
+  a.vec = a.vec && 2 * d->dim * es <= kNormRingMost;
+  a.error = device_error_word();
+  if (!a.error) return fail(BST_ERR_CUDA, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int tpr = norm_threads(d->dim);
   const int slots = tpr && tpr < 256 ? 256 / tpr : 1;
-  // Blocks that walk over the rows keep their parameters: as many as are resident (1024 threads per SM), long rows
-  // one block each.
-  const int64_t resident = tpr ? int64_t(sm_count()) * 1024 / std::max(tpr, 256) : INT_MAX;
-  const unsigned blocks = unsigned(std::min<int64_t>((d->rows + slots - 1) / slots, resident));
+  const int64_t blocks = (d->rows + slots - 1) / slots;
   return with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
     if (tpr) return norm_launch<T, false>(a, tpr, blocks, st);
-    norm_forward_long_kernel<T><<<blocks, 1024, 0, st>>>(a);
+    norm_forward_long_kernel<T><<<unsigned(std::min<int64_t>(blocks, INT_MAX)), 1024, 0, st>>>(a);
     return launched("norm_forward_long_kernel launch");
   });
 }
@@ -426,12 +576,15 @@ int bst_layer_norm_backward(const bst_norm_desc* d, const void* x, const void* w
   a.wide = d->param_dtype == BST_F32 && d->dtype != BST_F32;
   a.vec = aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(weight) && d->dim % per == 0 && d->x_row % per == 0 &&
           d->dy_row % per == 0 && d->dx_row % per == 0;
+  a.vec = a.vec && 4 * d->dim * es <= kNormRingMost;
   a.params = params;
+  a.error = device_error_word();
+  if (!a.error) return fail(BST_ERR_CUDA, "device error word unavailable");
   a.inv_dim = 1.f / float(d->dim);
   const int tpr = norm_threads(d->dim);
   int rc = with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
-    if (tpr) return norm_launch<T, true>(a, tpr, unsigned(norm_backward_blocks(d->rows, tpr)), st);
+    if (tpr) return norm_launch<T, true>(a, tpr, norm_backward_blocks(d->rows, tpr), st);
     norm_backward_long_kernel<T><<<unsigned(std::min<int64_t>(d->rows, INT_MAX)), 1024, 0, st>>>(a);
     if (int e = launched("norm_backward_long_kernel launch")) return e;
     if (!params) return int(BST_OK);
