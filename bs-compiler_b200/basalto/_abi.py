@@ -17,7 +17,7 @@ MAX_TERMS = 2304
 
 BST_OK, BST_ERR_INVALID, BST_ERR_UNSUPPORTED, BST_ERR_CUDA, BST_ERR_NCCL, BST_ERR_TIMEOUT, BST_ERR_NO_DEVICE = range(7)
 BST_F32, BST_F64, BST_BF16, BST_F16 = range(4)
-BST_SCAN_FORWARD, BST_SCAN_BACKWARD, BST_SCAN_SAVED = range(3)
+BST_SCAN_BACKWARD, BST_SCAN_SAVED = 1, 2
 BST_PROGRAM_CONTRACT = 1  # program flag: fold later multiplied terms with fma
 TERM_SUM, TERM_MUL, TERM_DIV = 0, 1, 2
 BOUNDARY_ZERO, BOUNDARY_VALID = 0, 1
@@ -139,7 +139,7 @@ SIGNATURES = [
     ("bst_causal_conv_step", c_int32,
      [POINTER(CConvDesc), c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     ("bst_scan_workspace", c_int32, [POINTER(CScanDesc), c_int32, POINTER(c_int64)]),
-    ("bst_scan_forward", c_int32, [POINTER(CScanDesc)] + [c_void_p] * 14 + [c_int64, c_void_p]),
+    ("bst_scan_forward", c_int32, [POINTER(CScanDesc)] + [c_void_p] * 14),
     ("bst_scan_backward", c_int32, [POINTER(CScanDesc)] + [c_void_p] * 23 + [c_int64, c_void_p]),
     ("bst_scan_step", c_int32,
      [POINTER(CScanDesc)] + [c_void_p] * 9 + [c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),

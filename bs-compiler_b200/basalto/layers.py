@@ -36,12 +36,13 @@ def _type(name, t):
 
 def _need(name, what, t, shape, dtype, device):
     """`t` is a tensor of this shape, element type and device."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"basalto.{name}: {what} must have shape {shape}, got {tuple(t.shape)}")
+    if t.shape == shape and t.dtype == dtype and t.device == device:
+        return
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"basalto.{name}: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise TypeError(f"basalto.{name}: {what} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise RuntimeError(f"basalto.{name}: {what} is on {t.device}, the input on {device}")
+    raise RuntimeError(f"basalto.{name}: {what} is on {t.device}, the input on {device}")
 
 
 def _cuda(name, t):
@@ -89,7 +90,11 @@ def _lengths(name, lengths, batch, device):
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _on(stream, fn, *args):
@@ -342,7 +347,7 @@ def _out_state(name, state, out_state):
     """The tensor that receives the new state: `state` itself, or a buffer that shares no memory with it."""
     if out_state is None or out_state is state:
         return state
-    _need(name, "out_state", out_state, tuple(state.shape), state.dtype, state.device)
+    _need(name, "out_state", out_state, state.shape, state.dtype, state.device)
     if state.numel() and out_state.data_ptr() == state.data_ptr() and out_state.stride() == state.stride():
         return out_state
     if state.numel() and _spans_meet(state, out_state):
@@ -368,13 +373,14 @@ def _distinct(name, what, t):
             reach += (n - 1) * s
 
 
-@torch.compiler.disable
 def causal_conv_step(x, state, weight, bias=None, activation=None, out_state=None, stream=None):
     """One position of causal_conv for every sequence: x [batch, channels], state [batch, width - 1, channels]
     (oldest input first) -> (y [batch, channels], new state).
 
     The new state replaces `state` in place, or goes to `out_state` (which shares no memory with it).  The state's
     rows are contiguous; sequences may lie at any distance."""
+    if torch.compiler.is_compiling():
+        return _eager_conv_step(x, state, weight, bias, activation, out_state, stream)
     name = "causal_conv_step"
     code = _type(name, x)
     _cuda(name, x)
@@ -402,6 +408,9 @@ def causal_conv_step(x, state, weight, bias=None, activation=None, out_state=Non
     if rc:
         _abi.check(rc)
     return y, out
+
+
+_eager_conv_step = torch.compiler.disable(causal_conv_step)
 
 
 # ---- selective scan ----------------------------------------------------------------------------
@@ -436,11 +445,9 @@ def _scan_forward(u, delta, A, B, C, D, z, bias, softplus, initial, lengths, wan
         saved = None
         if want_saved:
             saved = torch.empty(_rust.scan_workspace(*head, _abi.BST_SCAN_SAVED), dtype=torch.uint8, device=dev)
-        room = _rust.scan_workspace(*head, _abi.BST_SCAN_FORWARD)
-        ws = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
         rc = _rust.scan_forward(*head, u.data_ptr(), delta.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(),
                                 _ptr(D), _ptr(z), _ptr(bias), _ptr(initial), _ptr(lengths), y.data_ptr(), _ptr(final),
-                                _ptr(saved), _ptr(ws), room, _stream(u))
+                                _ptr(saved), _stream(u))
     if rc:
         _abi.check(rc)
     return y, final, saved
@@ -501,9 +508,9 @@ def _scan_args(name, u, delta, A, B, C, D, z, delta_bias):
     n = A.shape[1]
     f32, dev = torch.float32, u.device
     _need(name, "A", A, (c, n), f32, dev)
-    _need(name, "delta", delta, tuple(u.shape), u.dtype, dev)
+    _need(name, "delta", delta, u.shape, u.dtype, dev)
     if z is not None:
-        _need(name, "z", z, tuple(u.shape), u.dtype, dev)
+        _need(name, "z", z, u.shape, u.dtype, dev)
     if D is not None:
         _need(name, "D", D, (c,), f32, dev)
     if delta_bias is not None:
@@ -566,7 +573,6 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     return (y, final) if return_state else y
 
 
-@torch.compiler.disable
 def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=None, delta_softplus=False,
                         out_state=None, stream=None):
     """One position of selective_scan for every sequence: u, delta, z [batch, channels], B, C [batch, states] or
@@ -574,6 +580,8 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
 
     The new state replaces `state` in place, or goes to `out_state` (which shares no memory with it).  The state's
     last axis is contiguous; sequences and channels may lie at any distance."""
+    if torch.compiler.is_compiling():
+        return _eager_scan_step(u, delta, A, B, C, state, D, z, delta_bias, delta_softplus, out_state, stream)
     name = "selective_scan_step"
     code = _type(name, u)
     _cuda(name, u)
@@ -603,3 +611,6 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     if rc:
         _abi.check(rc)
     return y, out
+
+
+_eager_scan_step = torch.compiler.disable(selective_scan_step)

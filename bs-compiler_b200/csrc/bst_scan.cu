@@ -38,10 +38,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
   const int c0 = at.ct * CT, left = a.per_group - c0;  // channels of the group from this tile on
   const int64_t cbase = int64_t(at.g) * a.per_group + c0;
   const int64_t len = scan_length(a, at.b);
-  const int64_t first = int64_t(at.seg) * a.seg_tiles * kScanTile;
-  const int64_t stop = min(first + int64_t(a.seg_tiles) * kScanTile, a.length);  // of this segment
-  const int64_t live = max(min(stop, len), first);
-  const int tiles = int((live - first + kScanTile - 1) / kScanTile);
+  const int tiles = int((len + kScanTile - 1) / kScanTile);
 
   if (threadIdx.x < NT) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -60,7 +57,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
     for (int k = 0, slot = 0; k < tiles; ++k, slot = slot + 1 == SLOTS ? 0 : slot + 1) {
       const int buf = k & 1;
       if (a.saved) {
-        float* p = a.saved + ((at.b * ((a.length + kScanTile - 1) / kScanTile) + first / kScanTile + k) * a.channels +
+        float* p = a.saved + ((at.b * ((a.length + kScanTile - 1) / kScanTile) + k) * a.channels +
                               cbase + c_lane) * NP + sg * S;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -121,7 +118,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
         }
       bar_arrive<2 * NT, kDone>(buf);
     }
-    if (a.final_state && at.seg == a.segments - 1) {
+    if (a.final_state) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -159,7 +156,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
       if constexpr (TILES) {
         if (me == 0) {
           uint64_t* bar = &raw.bar[next_slot];
-          const int t = int(first) + next * kScanTile, c = int(cbase), b = int(at.b);
+          const int t = next * kScanTile, c = int(cbase), b = int(at.b);
           mbar_expect_tx(bar, unsigned((a.z ? 3 : 2) * sizeof(act[0]) + sizeof(bc)));
           tma_load_3d(&act[0][0][0], &maps.u, bar, c, t, b);
           tma_load_3d(&act[1][0][0], &maps.delta, bar, c, t, b);
@@ -168,8 +165,8 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
           tma_load_4d(&bc[1][0][0], &maps.C, bar, 0, at.g, t, b);
         }
       } else {
-        const int64_t t0 = first + int64_t(next) * kScanTile;
-        const int rows = int(min(live - t0, int64_t(kScanTile)));
+        const int64_t t0 = int64_t(next) * kScanTile;
+        const int rows = int(min(len - t0, int64_t(kScanTile)));
         const bool words = a.mode == kCopyWords;
         auto stage = [&](auto width, T* to, const void* p, int64_t off, int64_t st, int n) {
           stage_tile<T, decltype(width)::value, NT>(to, static_cast<const T*>(p) + off + t0 * st, st, rows, n, words, me);
@@ -206,7 +203,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
   // lies behind the end is cleared on the way, so that it meets the recurrences as zeros.
   auto convert = [&](int k, int slot) {
     Steps s;
-    const int rows = int(min(live - first - int64_t(k) * kScanTile, int64_t(kScanTile)));
+    const int rows = int(min(len - int64_t(k) * kScanTile, int64_t(kScanTile)));
     // Every branch stands outside of the loops over the turns, whose latencies then overlap.
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) s.d[i] = add2(load_pair(&raw.act[slot][1][Share::row(i)][col]), bias);
@@ -250,7 +247,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
   int slot = 0, ahead = 2, turn = 0;  // slots of tile k and k + 2, and the latter's turn
   for (int k = 0; k < tiles; ++k) {
     const int buf = k & 1;
-    const int64_t t0 = first + int64_t(k) * kScanTile;
+    const int64_t t0 = int64_t(k) * kScanTile;
     // While the recurrences of tile k run: D u and the gate of tile k, the step sizes of tile k + 2.
     float2 v[TURNS], g[TURNS];
 #pragma unroll
@@ -279,7 +276,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) v[i] = a.z ? mul2(v[i], g[i]) : v[i];
     T* row = y + (t0 + me / Share::PAIRS) * a.ys;
-    if (a.vec && in1 && t0 + kScanTile <= live) {
+    if (a.vec && in1 && t0 + kScanTile <= len) {
 #pragma unroll
       for (int i = 0; i < TURNS; ++i)
         *reinterpret_cast<Chunk<T, 2>*>(row + i * Share::ROWS * a.ys) = to_pair<T>(v[i]);
@@ -287,8 +284,8 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int64_t t = t0 + Share::row(i);
-        if (t < stop)
-          store_chunk<T, 2>(row + i * Share::ROWS * a.ys, to_pair<T>(t < live ? v[i] : both(0.f)), left - col, false);
+        if (t < a.length)
+          store_chunk<T, 2>(row + i * Share::ROWS * a.ys, to_pair<T>(t < len ? v[i] : both(0.f)), left - col, false);
       }
     }
     slot = slot + 1 == SLOTS ? 0 : slot + 1;
@@ -297,7 +294,7 @@ __global__ void __launch_bounds__(2 * Sh::NT, 2)
   if (TILES && failed)  // copies that are late may not outlive the block
     for (int i = 0; i < SLOTS; ++i) mbar_wait_bounded(&raw.bar[i], unsigned((next - 1 - i) / SLOTS) & 1u);
   // Positions behind the sequence's end.
-  for (int64_t t = first + int64_t(tiles) * kScanTile + me / Share::PAIRS; t < stop; t += Share::ROWS)
+  for (int64_t t = int64_t(tiles) * kScanTile + me / Share::PAIRS; t < a.length; t += Share::ROWS)
     store_chunk<T, 2>(y + t * a.ys, to_pair<T>(both(0.f)), left - col, a.vec);
 }
 
@@ -321,8 +318,6 @@ ScanArgs scan_args(const bst_scan_desc* d) {
   a.length = d->length, a.channels = int(d->channels), a.groups = int(d->groups);
   a.per_group = int(d->channels / d->groups), a.states = int(d->states), a.batch = int(d->batch);
   a.softplus = d->softplus != 0;
-  a.segments = 1;
-  a.seg_tiles = int((d->length + kScanTile - 1) / kScanTile);
   return a;
 }
 
@@ -396,7 +391,7 @@ bool scan_maps(const bst_scan_desc* d, int tile_channels, int pad, const void* u
 template <typename T, class Sh>
 static int scan_forward_launch(const bst_scan_desc* d, ScanArgs a, cudaStream_t st) {
   a.col_tiles = (a.per_group + Sh::CT - 1) / Sh::CT;
-  const int64_t blocks = int64_t(a.batch) * a.segments * a.groups * a.col_tiles;
+  const int64_t blocks = int64_t(a.batch) * a.groups * a.col_tiles;
   if (blocks > INT_MAX) return fail(BST_ERR_UNSUPPORTED, "the scan needs more than 2^31 blocks");
   ScanMaps maps;
   if (a.mode == kCopyTiles && !scan_maps(d, Sh::CT, Sh::NP, a.u, a.delta, a.z, nullptr, a.B, a.C, &maps))
@@ -418,8 +413,7 @@ int bst_scan_workspace(const bst_scan_desc* d, int32_t what, int64_t* bytes) {
   clear_error();
   if (int rc = scan_check(d)) return rc;
   if (!bytes) return fail(BST_ERR_INVALID, "null output");
-  if (what == BST_SCAN_FORWARD) *bytes = 0;
-  else if (what == BST_SCAN_BACKWARD) *bytes = scan_backward_workspace(d);
+  if (what == BST_SCAN_BACKWARD) *bytes = scan_backward_workspace(d);
   else if (what == BST_SCAN_SAVED) *bytes = scan_saved_bytes(d);
   else return fail(BST_ERR_INVALID, "unknown workspace");
   return BST_OK;
@@ -427,10 +421,9 @@ int bst_scan_workspace(const bst_scan_desc* d, int32_t what, int64_t* bytes) {
 
 int bst_scan_forward(const bst_scan_desc* d, const void* u, const void* delta, const float* A, const void* B,
                      const void* C, const float* D, const void* z, const float* delta_bias, const float* initial,
-                     const int32_t* lengths, void* y, float* final_state, void* saved, void* workspace,
-                     int64_t workspace_bytes, void* stream) {
-  int64_t need = 0;
-  if (int rc = bst_scan_workspace(d, BST_SCAN_FORWARD, &need)) return rc;
+                     const int32_t* lengths, void* y, float* final_state, void* saved, void* stream) {
+  clear_error();
+  if (int rc = scan_check(d)) return rc;
   if (d->batch == 0 || d->channels == 0) return BST_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d->length == 0) {  // the state passes through
@@ -441,8 +434,7 @@ int bst_scan_forward(const bst_scan_desc* d, const void* u, const void* delta, c
     return BST_OK;
   }
   if (!u || !delta || !A || !B || !C || !y) return fail(BST_ERR_INVALID, "null device pointer");
-  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-    return fail(BST_ERR_INVALID, "the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
+  if (!aligned16(saved)) return fail(BST_ERR_INVALID, "the saved states must be aligned to 16 bytes");
   ScanArgs a = scan_args(d);
   a.u = u, a.delta = delta, a.A = A, a.B = B, a.C = C, a.D = D, a.z = z, a.dbias = delta_bias, a.init = initial;
   a.lengths = lengths, a.y = y, a.final_state = final_state, a.saved = static_cast<float*>(saved);
@@ -454,18 +446,21 @@ int bst_scan_forward(const bst_scan_desc* d, const void* u, const void* delta, c
   if (!a.error) return fail(BST_ERR_CUDA, "device error word unavailable");
   return with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
-    // Two channels per lane halve the shared-memory bytes and the sums' shuffles per recurrence; one channel
-    // doubles the warps.  Two pay from about one warp per scheduler on.  16 states, bf16, one | two channels:
-    // 1 x 4096 x 4096 186 | 283 us, 4 x 2048 x 4096 305 | 250 us.
-    const bool wide = d->batch * d->channels * scan_pad(d->states) >= int64_t(sm_count()) * 4 * 256;
+    // Two channels per lane halve the shared-memory bytes and the sums' shuffles per recurrence; one channel, or one
+    // with half of the states, doubles the warps each time, which pays while they are scarce.  By channel-state pairs
+    // per scheduler of the GPU; with 16 states in bf16, 2 channels x 4 states | 1 x 4 | 1 x 2 per lane:
+    // 4 x 2048 x 4096: 324 | 410 | 426 us, 1 x 4096 x 8192: 370 | 414 | 503, 1 x 4096 x 4096: 364 | 261 | 268,
+    // 1 x 4096 x 1024: 361 | 256 | 174.
+    const int64_t pairs = d->batch * d->channels * scan_pad(d->states) / (int64_t(sm_count()) * 4);
     switch (scan_pad(d->states)) {
       case 4: return scan_forward_launch<T, ScanShape<2, 2, 2, 2>>(d, a, st);
       case 8: return scan_forward_launch<T, ScanShape<4, 2, 2, 2>>(d, a, st);
       case 16:
-        if (wide) return scan_forward_launch<T, ScanShape<4, 2, 4, 4>>(d, a, st);
-        return scan_forward_launch<T, ScanShape<4, 1, 4, 4>>(d, a, st);
+        if (pairs >= 192) return scan_forward_launch<T, ScanShape<4, 2, 4, 4>>(d, a, st);
+        if (pairs >= 64) return scan_forward_launch<T, ScanShape<4, 1, 4, 4>>(d, a, st);
+        return scan_forward_launch<T, ScanShape<2, 1, 8, 4>>(d, a, st);
       case 32:
-        if (wide) return scan_forward_launch<T, ScanShape<4, 2, 8, 4>>(d, a, st);
+        if (pairs >= 192) return scan_forward_launch<T, ScanShape<4, 2, 8, 4>>(d, a, st);
         return scan_forward_launch<T, ScanShape<4, 1, 8, 4>>(d, a, st);
       default: return scan_forward_launch<T, ScanShape<4, 2, 16, 4>>(d, a, st);
     }

@@ -9,8 +9,9 @@
 // fp32 instructions, whose B and C operands then lie in shared memory as they are, while the two numbers of
 // a channel (d and d u) are doubled in registers: a shared-memory load costs by the bytes that its lanes
 // receive, broadcast or not.  A warp steps through the sequence in order.  Sequences come in tiles of 16
-// steps: a block loads a tile of u, delta (z, dy) for its channels and of B, C, computes what is shared
-// by the states (the step size) once, and leaves it in shared memory as the steps want it.
+// steps: a block copies a tile of u, delta (z, dy) for its channels and of B, C into shared memory as they
+// are, and computes what is shared by the states (the step size) once.  No store to shared memory stands
+// between the steps' loads: the loads of later steps would wait behind it.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -30,16 +31,15 @@ struct ScanArgs {
   const int* lengths;
   void *y, *du, *ddelta, *dz, *dB, *dC;
   float *final_state, *saved, *dinit;
-  float *seg_state, *seg_sum;    // [batch][segments][channels][NP] and [batch][segments][channels]
   float *part_bc;                // [batch][groups][tiles of channels][length][2 NP]
-  float *part_a, *part_d;        // [batch][segments][channels][NP], [batch][segments][channels][2]
+  float *part_a, *part_d;        // [batch][channels][NP], [batch][channels][2]
   int64_t ub, us, db, ds, zb, zs, yb, ys, dyb, dys, Bb, Bs, Bg, Cb, Cs, Cg;
   int64_t length;
   int channels, per_group, groups, states, batch;
   int softplus, vec;
   int mode;         // CopyMode of the inputs
   unsigned* error;  // the device's error word
-  int segments, seg_tiles, col_tiles;  // segments per sequence, 16-step tiles per segment, channel tiles per group
+  int col_tiles;    // channel tiles per group
 };
 
 // Geometry of a block's work: S states and CH channels per lane, GS lanes per channel, W warps.
@@ -61,7 +61,7 @@ __device__ __forceinline__ int64_t scan_length(const ScanArgs& a, int64_t b) {
 // Where a block works.
 struct ScanWhere {
   int64_t b;
-  int seg, g, ct;
+  int g, ct;
 };
 __device__ __forceinline__ ScanWhere scan_where(const ScanArgs& a) {
   ScanWhere w;
@@ -69,9 +69,7 @@ __device__ __forceinline__ ScanWhere scan_where(const ScanArgs& a) {
   w.ct = int(i % a.col_tiles);
   i /= a.col_tiles;
   w.g = int(i % a.groups);
-  i /= a.groups;
-  w.seg = int(i % a.segments);
-  w.b = i / a.segments;
+  w.b = i / a.groups;
   return w;
 }
 
@@ -180,23 +178,21 @@ __device__ __forceinline__ Chunk<T, 2> to_pair(float2 v) {
   return c;
 }
 
-// a_t of two states; a2 = A log2(e).
-__device__ __forceinline__ float2 decay(float2 step, float2 a2) { return ex2_2(mul2(step, a2)); }
-
-// What the states of CH neighbouring channels share at one step.
-template <int CH>
-struct alignas(8 * CH) Step {
-  float d[CH], du[CH];
-};
-
-// Step sizes d and d u of a pair of channels (col even), into a row of the tile's shared memory.
-template <int CH>
-__device__ __forceinline__ void put_steps(Step<CH>* row, int col, float2 d, float2 du) {
-  if constexpr (CH == 2) *reinterpret_cast<float4*>(&row[col / 2]) = make_float4(d.x, d.y, du.x, du.y);
-  else *reinterpret_cast<float4*>(&row[col]) = make_float4(d.x, du.x, d.y, du.y);
+// a_t = 2^x of two states, x = d A log2(e).  The special-function unit's 2^x is good to 2^-22.5; where a_t is near 1 a
+// state remembers 1 / (1 - a_t) steps and gathers as many of those errors (the gradient of A lost a digit to it), so
+// |x| < 1/16 takes the power series of e^t, t = x ln 2, |t| < 0.0434, up to t^4 / 24 (the rest is below t^5 / 120 =
+// 1.3e-9): its one rounding at 1 is that of the last fused operation.
+__device__ __forceinline__ float2 decay(float2 step, float2 a2) {
+  const float2 x = mul2(step, a2), m = ex2_2(x);
+  constexpr float c1 = kLn2, c2 = kLn2 * kLn2 / 2, c3 = kLn2 * kLn2 * kLn2 / 6, c4 = kLn2 * kLn2 * kLn2 * kLn2 / 24;
+  float2 p = fma2(both(c4), x, both(c3));
+  p = fma2(p, x, both(c2));
+  p = fma2(p, x, both(c1));
+  p = fma2(p, x, both(1.f));
+  return make_float2(fabsf(x.x) < 0.0625f ? p.x : m.x, fabsf(x.y) < 0.0625f ? p.y : m.y);
 }
 
-// Host: states per lane and the group count for N states.
+// N states padded to what the lanes of a channel hold.
 inline int scan_pad(int64_t n) {
   int p = 4;
   while (p < n) p *= 2;
@@ -212,6 +208,5 @@ bool scan_maps(const bst_scan_desc* d, int tile_channels, int pad, const void* u
 int scan_check(const bst_scan_desc* d);
 ScanArgs scan_args(const bst_scan_desc* d);
 int64_t scan_saved_bytes(const bst_scan_desc* d);
-int scan_segments(const bst_scan_desc* d, bool backward, int* tiles);
 
 }  // namespace bst

@@ -44,10 +44,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
   const int c0 = at.ct * CT, left = a.per_group - c0, cols = left < CT ? left : CT;
   const int64_t cbase = int64_t(at.g) * a.per_group + c0;
   const int64_t len = scan_length(a, at.b);
-  const int64_t first = int64_t(at.seg) * a.seg_tiles * kScanTile;
-  const int64_t stop = min(first + int64_t(a.seg_tiles) * kScanTile, a.length);
-  const int64_t live = max(min(stop, len), first);
-  const int tiles = int((live - first + kScanTile - 1) / kScanTile);
+  const int tiles = int((len + kScanTile - 1) / kScanTile);
 
   const int c_lane = CH * cell;
   Pairs<S> carry[CH], a2[CH], dA[CH];  // carry: a_{t+1} g_{t+1}
@@ -76,7 +73,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
   float* part = a.part_bc + ((at.b * a.groups + at.g) * a.col_tiles + at.ct) * a.length * 2 * NP;
 
   // Positions behind the sequence's end.
-  for (int64_t t = first + int64_t(tiles) * kScanTile + row0; t < stop; t += ROWS) {
+  for (int64_t t = int64_t(tiles) * kScanTile + row0; t < a.length; t += ROWS) {
     const Chunk<T, 2> zero = to_pair<T>(both(0.f));
     store_chunk<T, 2>(du + t * a.channels, zero, left - col, a.vec);
     store_chunk<T, 2>(ddl + t * a.channels, zero, left - col, a.vec);
@@ -96,7 +93,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
     if (k >= 0) {
       auto& act = m.act[slot];
       auto& bc = m.bc[slot];
-      const int64_t t0 = first + int64_t(k) * kScanTile;
+      const int64_t t0 = int64_t(k) * kScanTile;
       if constexpr (TILES) {
         if (threadIdx.x == 0) {
           uint64_t* bar = &m.bar[slot];
@@ -110,7 +107,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
           tma_load_4d(&bc[1][0][0], &maps.C, bar, 0, at.g, t, b);
         }
       } else {
-        const int rows = int(min(live - t0, int64_t(kScanTile))), me = threadIdx.x;
+        const int rows = int(min(len - t0, int64_t(kScanTile))), me = threadIdx.x;
         const bool words = a.mode == kCopyWords;
         auto stage = [&](auto width, T* to, const void* p, int64_t off, int64_t st, int n) {
           stage_tile<T, decltype(width)::value, NT>(to, static_cast<const T*>(p) + off + t0 * st, st, rows, n, words, me);
@@ -130,8 +127,8 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
   fetch(tiles - 1, 0);
   int slot = 0, turn = 0;
   for (int k = tiles - 1; k >= 0; --k) {
-    const int64_t t0 = first + int64_t(k) * kScanTile;
-    const int rows = int(min(live - t0, int64_t(kScanTile)));
+    const int64_t t0 = int64_t(k) * kScanTile;
+    const int rows = int(min(len - t0, int64_t(kScanTile)));
     Pairs<S> h0[CH], h[kScanTile][CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -337,7 +334,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
         const float2 dd = r < rows ? mul2(slope[i], fma2(w, both(kLn2), mul2(g[i], x[i]))) : both(0.f);
         dD = fma2(e, x[i], dD);
         dbias = make_float2(dbias.x + dd.x, dbias.y + dd.y);
-        if (t < stop) {
+        if (t < a.length) {
           store_chunk<T, 2>(du + t * a.channels, to_pair<T>(fma2(d, g[i], mul2(skip, e))), left - col, a.vec);
           store_chunk<T, 2>(ddl + t * a.channels, to_pair<T>(dd), left - col, a.vec);
         }
@@ -354,7 +351,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
           const int64_t t = t0 + row0 + i * ROWS;
-          if (t < stop) store_chunk<T, 2>(dz + t * a.channels, to_pair<T>(y[i]), left - col, a.vec);
+          if (t < a.length) store_chunk<T, 2>(dz + t * a.channels, to_pair<T>(y[i]), left - col, a.vec);
         }
       }
     }
@@ -372,7 +369,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
   if (TILES && failed)  // copies that are late may not outlive the block
     for (int i = 0; i < 2; ++i) mbar_wait_bounded(&m.bar[i], unsigned(turn) & 1u);
 
-  if (a.dinit && at.seg == 0) {
+  if (a.dinit) {
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -383,7 +380,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
               s % 2 ? carry[c].v[s / 2].y : carry[c].v[s / 2].x;
       }
   }
-  const int64_t prow = (at.b * a.segments + at.seg) * a.channels + cbase;
+  const int64_t prow = at.b * a.channels + cbase;
 #pragma unroll
   for (int c = 0; c < CH; ++c)
     if (c_lane + c < left) *reinterpret_cast<Pairs<S>*>(a.part_a + (prow + c_lane + c) * NP + sg * S) = dA[c];
@@ -434,7 +431,7 @@ __global__ void __launch_bounds__(256) scan_bc_kernel(const ScanArgs a, int np) 
   out[((b * a.length + t) * a.groups + g) * a.states + n] = from_f<T>(v);
 }
 
-// dA, dD, ddelta_bias: sums over the sequences (and their segments).
+// dA, dD, ddelta_bias: sums over the sequences.
 __global__ void __launch_bounds__(256) scan_params_kernel(const ScanArgs a, int np, int rows, float* dA, float* dD,
                                                           float* dbias) {
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
@@ -469,23 +466,23 @@ static auto with_backward_shape(int64_t states, F&& f) {
 struct BackwardLayout {
   int64_t bc, pa, pd, total;  // byte offsets of part_bc (0), part_a, part_d
 };
-static BackwardLayout backward_layout(const bst_scan_desc* d, int segments) {
+static BackwardLayout backward_layout(const bst_scan_desc* d) {
   const int64_t np = scan_pad(d->states);
   const int64_t ct = with_backward_shape(d->states, [](auto sh) { return int64_t(decltype(sh)::CT); });
   const int64_t per_group = d->channels / d->groups, tiles = (per_group + ct - 1) / ct;
   BackwardLayout l{};
   l.pa = d->batch * d->groups * tiles * d->length * 2 * np * 4;
-  l.pd = l.pa + d->batch * segments * d->channels * np * 4;
-  l.total = l.pd + d->batch * segments * d->channels * 2 * 4;
+  l.pd = l.pa + d->batch * d->channels * np * 4;
+  l.total = l.pd + d->batch * d->channels * 2 * 4;
   return l;
 }
 
-int64_t scan_backward_workspace(const bst_scan_desc* d) { return backward_layout(d, 1).total; }
+int64_t scan_backward_workspace(const bst_scan_desc* d) { return backward_layout(d).total; }
 
 template <typename T, class Sh>
 static int scan_backward_launch(const bst_scan_desc* d, ScanArgs a, cudaStream_t st) {
   a.col_tiles = (a.per_group + Sh::CT - 1) / Sh::CT;
-  const int64_t blocks = int64_t(a.batch) * a.segments * a.groups * a.col_tiles;
+  const int64_t blocks = int64_t(a.batch) * a.groups * a.col_tiles;
   const int64_t outs = int64_t(a.batch) * a.length * a.groups * 2 * Sh::NP;
   if (blocks > INT_MAX || outs / 256 + 1 > INT_MAX)
     return fail(BST_ERR_UNSUPPORTED, "the scan's gradients need more than 2^31 blocks");
@@ -527,13 +524,14 @@ extern "C" int bst_scan_backward(const bst_scan_desc* d, const void* u, const vo
   }
   if (!u || !delta || !A || !B || !C || !dy || !saved || !du || !ddelta || !dB || !dC || (z && !dz))
     return fail(BST_ERR_INVALID, "null device pointer");
+  if (!aligned16(saved)) return fail(BST_ERR_INVALID, "the saved states must be aligned to 16 bytes");
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return fail(BST_ERR_INVALID, "the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
   ScanArgs a = scan_args(d);
   a.u = u, a.delta = delta, a.A = A, a.B = B, a.C = C, a.D = D, a.z = z, a.dbias = delta_bias, a.lengths = lengths;
   a.dy = dy, a.dfinal = dfinal, a.saved = static_cast<float*>(const_cast<void*>(saved));
   a.du = du, a.ddelta = ddelta, a.dB = dB, a.dC = dC, a.dz = z ? dz : nullptr, a.dinit = dinitial;
-  const BackwardLayout l = backward_layout(d, a.segments);
+  const BackwardLayout l = backward_layout(d);
   char* ws = static_cast<char*>(workspace);
   a.part_bc = reinterpret_cast<float*>(ws);
   a.part_a = reinterpret_cast<float*>(ws + l.pa);
@@ -552,6 +550,6 @@ extern "C" int bst_scan_backward(const bst_scan_desc* d, const void* u, const vo
   if (rc) return rc;
   const int np = scan_pad(d->states);
   const int64_t n = d->channels * (np + 2);
-  scan_params_kernel<<<unsigned((n + 255) / 256), 256, 0, st>>>(a, np, a.batch * a.segments, dA, dD, ddelta_bias);
+  scan_params_kernel<<<unsigned((n + 255) / 256), 256, 0, st>>>(a, np, a.batch, dA, dD, ddelta_bias);
   return launched("scan_params_kernel launch");
 }

@@ -169,12 +169,10 @@ int64_t scan_workspace(int dtype, int softplus, const ints& v, int what) {
   return n;
 }
 int scan_forward(int dtype, int softplus, const ints& v, addr u, addr delta, addr A, addr B, addr C, addr D, addr z,
-                 addr bias, addr init, addr lengths, addr y, addr final_state, addr saved, addr ws, int64_t bytes,
-                 addr stream) {
+                 addr bias, addr init, addr lengths, addr y, addr final_state, addr saved, addr stream) {
   const bst_scan_desc d = scan_desc(dtype, softplus, v);
   return bst_scan_forward(&d, at(u), at(delta), at<f32>(A), at(B), at(C), at<f32>(D), at(z), at<f32>(bias),
-                          at<f32>(init), at<int32_t>(lengths), at(y), at<f32>(final_state), at(saved), at(ws), bytes,
-                          at(stream));
+                          at<f32>(init), at<int32_t>(lengths), at(y), at<f32>(final_state), at(saved), at(stream));
 }
 int scan_backward(int dtype, int softplus, const ints& v, addr u, addr delta, addr A, addr B, addr C, addr D, addr z,
                   addr bias, addr lengths, addr dy, addr dfinal, addr saved, addr du, addr ddelta, addr dA, addr dB,

@@ -345,9 +345,11 @@ BST_API int bst_march_item_plan(int64_t tiles, int64_t planes, int32_t rb, int32
  * Element types: `dtype` (F32, BF16 or F16) for the activations; arithmetic, sums and
  * states are fp32, and each result is rounded once.  Strides are in elements; the innermost
  * axis of every tensor is contiguous unless stated otherwise.  Optional pointers are NULL
- * when absent.  Every call queues its kernels on `stream` of the current device, allocates
- * nothing and can be captured into a CUDA graph; workspaces are the caller's, must be aligned
- * to 16 bytes, and belong to one call at a time (two calls that may overlap need two).
+ * when absent.  Every call queues its kernels on `stream` of the current device and can be
+ * captured into a CUDA graph.  It allocates nothing, but for the first call on a device, which sets
+ * up the error word that bst_device_error_check reads and belongs before any capture.  Workspaces
+ * are the caller's, must be aligned to 16 bytes, and belong to one call at a time (two calls that
+ * may overlap need two).
  * Results do not depend on the order in which blocks run (no atomics).
  * Empty problems (no rows, no batch, no channels) return BST_OK; a reduction over nothing
  * (gradients of parameters) is then zero. */
@@ -412,20 +414,20 @@ BST_API int bst_causal_conv_step(const bst_conv_desc* d, const void* x, const vo
  * states], D, delta_bias [channels], initial and final [batch, channels, states]: fp32,
  * contiguous.  delta_bias, D, z, initial (zeros) and lengths (as above) are optional; final is
  * the state after lengths[b] steps.  states 1..64; groups divides channels.
- * A workspace of bst_scan_workspace(.., BST_SCAN_FORWARD) bytes may be needed.  `saved` (NULL,
- * or BST_SCAN_SAVED bytes) receives the states that the backward pass starts from. */
+ * `saved` (NULL, or BST_SCAN_SAVED bytes of bst_scan_workspace, aligned to 16) receives every 16th
+ * state; the backward pass starts from them. */
 typedef struct bst_scan_desc {
   int32_t dtype, softplus;
   int64_t batch, length, channels, states, groups;
   int64_t u_batch, u_step, delta_batch, delta_step, z_batch, z_step, y_batch, y_step, dy_batch, dy_step;
   int64_t B_batch, B_step, B_group, C_batch, C_step, C_group;
 } bst_scan_desc;
-enum { BST_SCAN_FORWARD = 0, BST_SCAN_BACKWARD = 1, BST_SCAN_SAVED = 2 };
+enum { BST_SCAN_BACKWARD = 1, BST_SCAN_SAVED = 2 };
 BST_API int bst_scan_workspace(const bst_scan_desc* d, int32_t what, int64_t* bytes);
 BST_API int bst_scan_forward(const bst_scan_desc* d, const void* u, const void* delta, const float* A, const void* B,
                              const void* C, const float* D, const void* z, const float* delta_bias,
                              const float* initial, const int32_t* lengths, void* y, float* final_state, void* saved,
-                             void* workspace, int64_t workspace_bytes, void* stream);
+                             void* stream);
 /* Gradients, contiguous: du, ddelta, dz [batch, length, channels] and dB, dC [batch, length,
  * groups, states] in dtype; dA, dD, ddelta_bias, dinitial in fp32.  dz, dD, ddelta_bias and
  * dinitial are optional; dfinal (optional) is the gradient of final.  Positions from

@@ -192,7 +192,7 @@ def test_c_entries_refuse_before_any_device_work():
                                         None) == _abi.BST_ERR_INVALID
 
     sd = _abi.CScanDesc(dtype=_abi.BST_F32, batch=2, length=5, channels=8, states=4, groups=3)
-    room = lambda what=0: lib.bst_scan_workspace(P(sd), what, P(n))  # noqa: E731
+    room = lambda what=1: lib.bst_scan_workspace(P(sd), what, P(n))  # noqa: E731
     assert room() == _abi.BST_ERR_INVALID  # groups do not divide the channels
     sd.groups = 2
     assert room() == _abi.BST_OK and room(7) == _abi.BST_ERR_INVALID
@@ -201,7 +201,7 @@ def test_c_entries_refuse_before_any_device_work():
     sd.states = 0
     assert room() == _abi.BST_ERR_UNSUPPORTED
     sd.states = 4
-    assert lib.bst_scan_forward(P(sd), *[None] * 14, 0, None) == _abi.BST_ERR_INVALID
+    assert lib.bst_scan_forward(P(sd), *[None] * 14) == _abi.BST_ERR_INVALID
     assert lib.bst_scan_step(P(sd), *[None] * 9, 0, 0, None, None, 0, 0, None) == _abi.BST_ERR_INVALID
 
 
