@@ -61,9 +61,17 @@ def _layer_norm(n):
     if x is None or not _usable(x) or not isinstance(eps, (int, float)):
         return None
     shape = (shape,) if isinstance(shape, int) else tuple(shape)
+    if not _keeps_type(n, x):
+        return None
     if x.dim() < 1 or shape != (x.shape[-1],) or not (_param_ok(w, x) and _param_ok(b, x) and _same_type(w, b)):
         return None
     return layers.layer_norm, (_arg(n, 0, "input"), w, b, float(eps))
+
+
+def _keeps_type(n, x):
+    """The node's result has its input's element type (autocast can make it another one: left alone)."""
+    v = _value(n)
+    return v is not None and v.dtype == x.dtype
 
 
 def _one(v, want):
@@ -87,7 +95,7 @@ def _causal_conv(n):
     if groups != c or tuple(wv.shape) != (c, 1, taps) or not 1 <= taps <= 8 or not (_one(stride, 1) and
                                                                                     _one(dilation, 1)):
         return None
-    if not (_param_ok(w, xv) and _param_ok(b, xv) and _same_type(w, b)):
+    if not (_param_ok(w, xv) and _param_ok(b, xv) and _same_type(w, b) and _keeps_type(n, xv)):
         return None
     if _one(pad, 0) and isinstance(x, torch.fx.Node) and x.target in _PAD and x.op == "call_function":
         spec = tuple(_arg(x, 1, "pad"))

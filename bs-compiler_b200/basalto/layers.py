@@ -97,6 +97,11 @@ def _wants_grad(*ts):
     return False
 
 
+def _no_stream(name, stream):
+    if stream is not None:
+        raise RuntimeError(f"basalto.{name}: stream= is not available in compiled graphs")
+
+
 def _on(stream, fn, *args):
     """fn(*args) with `stream` current; the caching allocator learns that the inputs are used there."""
     with torch.cuda.stream(stream):
@@ -190,6 +195,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stream=None):
             _param(name, what, p, (x.shape[-1],), x)
     _same_params(name, weight, bias)
     if torch.compiler.is_compiling():
+        _no_stream(name, stream)
         return torch.ops.basalto.layer_norm(x, weight, bias, eps)[0]
     _cuda(name, x)
     if stream is not None:
@@ -324,6 +330,7 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, lengt
         _need(name, "initial_state", initial_state, (b, weight.shape[1] - 1, c), x.dtype, x.device)
     lengths = _lengths(name, lengths, b, x.device)
     if torch.compiler.is_compiling():
+        _no_stream(name, stream)
         y, final = torch.ops.basalto.causal_conv(x, weight, bias, bool(silu), initial_state, lengths)
         return (y, final) if return_state else y
     _cuda(name, x)
@@ -554,6 +561,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
         _need(name, "initial_state", initial_state, (b, c, A.shape[1]), torch.float32, u.device)
     lengths = _lengths(name, lengths, b, u.device)
     if torch.compiler.is_compiling():
+        _no_stream(name, stream)
         save = _wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state)
         y, final, _ = torch.ops.basalto.selective_scan(u, delta, A, B, C, D, z, delta_bias, bool(delta_softplus),
                                                        initial_state, lengths, save)

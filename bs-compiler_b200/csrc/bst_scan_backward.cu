@@ -9,9 +9,14 @@
 //
 // The states are needed backwards and kept nowhere: the forward pass saved every 16th, and a block
 // recomputes the 16 of a tile from it into registers, walking the tiles from the last to the first.
-// Two exponentials for each (position, channel, state) bound it, and the sums over states and over
-// channels that each step asks for: they go through reduce_scatter over the lanes, dB and dC then
-// through shared memory over the block's warps and through a partial array over the channel tiles.
+// Two exponentials for each (position, channel, state) and the sums over states and over channels that
+// each step asks for bound it: they go through reduce_scatter over the lanes, dB and dC then through
+// shared memory over the block's warps and through a partial array over the channel tiles.
+//
+// Measured on B200, 4 x 2048 x 4096 with 16 states in bf16: 1020 us and 17 us for the sums over the channel tiles
+// (29 instructions per (position, channel, state) before the series near 1 was added, schedulers 50 % busy at two
+// warps each: the 16 states of a tile take 128 registers).  One channel per lane, or two states, halve those and
+// double the warps, but need more instructions for each: 1125 and 1046 us against 886 us then.
 #include <algorithm>
 
 #include "bst_scan.cuh"

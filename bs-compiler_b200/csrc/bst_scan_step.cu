@@ -2,7 +2,8 @@
 //
 //   h' = exp(d A) h + d u B,   y = (sum_n C h' + D u) silu(z)
 // The state is read and written once in fp32 (8 bytes per entry) and dwarfs everything else, so HBM
-// bounds it; with a few sequences the launch does.  L lanes share a channel, each with vectors of V
+// bounds it; with a few sequences the launch does (256 x 4096 x 16 in bf16: 36 us on B200 for 143 MB, 3.9 TB/s of
+// a plain copy's 6.55; 2 x 1030 x 24 in fp32: 2.2 us).  L lanes share a channel, each with vectors of V
 // states, and reduce y over themselves; a thread has read its states before it writes them, so that
 // out_state may be the state itself.
 #include <algorithm>
@@ -115,7 +116,7 @@ extern "C" int bst_scan_step(const bst_scan_desc* d, const void* u, const void* 
   return with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
     using std::integral_constant;
-    // Four sequences per thread where that leaves two full turns of blocks (256 x 4096 x 16: 57 us with one, 25 with
+    // Four sequences per thread where that leaves two full turns of blocks (256 x 4096 x 16: 57 us with one, 36 with
     // four), one where threads are scarce.
     auto go = [&](auto lc, auto vc, auto kc) {
       constexpr int L = decltype(lc)::value, V = decltype(vc)::value, K = decltype(kc)::value;

@@ -350,6 +350,7 @@ BST_API int bst_march_item_plan(int64_t tiles, int64_t planes, int32_t rb, int32
  * up the error word that bst_device_error_check reads and belongs before any capture.  Workspaces
  * are the caller's, must be aligned to 16 bytes, and belong to one call at a time (two calls that
  * may overlap need two).
+ * Up to 65535 sequences per call of the convolution and of the steps, 2^24 of the scan.
  * Results do not depend on the order in which blocks run (no atomics).
  * Empty problems (no rows, no batch, no channels) return BST_OK; a reduction over nothing
  * (gradients of parameters) is then zero. */

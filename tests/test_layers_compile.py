@@ -88,6 +88,16 @@ def test_leaves_cpu_tensors_and_other_convolutions_alone():
     assert fx_layers.route(as_cuda(graph_of(Block(dtype=torch.float64), double))) == 0
 
 
+def test_leaves_autocast_regions_alone():
+    """Under autocast a layer norm answers in fp32 and a convolution in bf16, whatever their input's type."""
+    m = Block()
+    gm = as_cuda(graph_of(m, torch.randn(2, L, C)))
+    for n in gm.graph.nodes:
+        if n.op == "call_function" and n.target in (F.layer_norm, torch.conv1d, F.conv1d):
+            n.meta["example_value"] = n.meta["example_value"].to(torch.bfloat16)
+    assert fx_layers.route(gm) == 0
+
+
 def test_off_by_default(monkeypatch):
     monkeypatch.delenv("BASALTO_MODEL_OPS", raising=False)
     m = Block()
