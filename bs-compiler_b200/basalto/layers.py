@@ -355,6 +355,8 @@ def _out_state(name, state, out_state):
     if out_state is None or out_state is state:
         return state
     _need(name, "out_state", out_state, state.shape, state.dtype, state.device)
+    if state.untyped_storage().data_ptr() != out_state.untyped_storage().data_ptr():
+        return out_state
     if state.numel() and out_state.data_ptr() == state.data_ptr() and out_state.stride() == state.stride():
         return out_state
     if state.numel() and _spans_meet(state, out_state):
@@ -611,8 +613,9 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     A, D, delta_bias = A.contiguous(), _dense(D), _dense(delta_bias)
     y = torch.empty(b, c, dtype=u.dtype, device=u.device)
     with _guard(u):
+        (Bb, Bg, _), (Cb, Cg, _) = B.stride(), C.stride()
         rc = _rust.scan_step(code, 1 if delta_softplus else 0, b, c, n, B.shape[1], u.stride(0), delta.stride(0),
-                             0 if z is None else z.stride(0), c, B.stride(0), B.stride(1), C.stride(0), C.stride(1),
+                             0 if z is None else z.stride(0), c, Bb, Bg, Cb, Cg,
                              u.data_ptr(), delta.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(D),
                              _ptr(z), _ptr(delta_bias), state.data_ptr(), state.stride(0), state.stride(1),
                              y.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), _stream(u))

@@ -31,24 +31,13 @@ __device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16_
 template <>
 __device__ __forceinline__ fp16 from_f<fp16>(float v) { return __float2half_rn(v); }
 
-// V elements that move as one access when `vec` (the caller has checked alignment), else one by one.
+// V elements that move as one access.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Chunk {
   T v[V];
 };
 
-// Elements [0, n) of p (n <= 0: none); the others read zero.
-template <typename T, int V>
-__device__ __forceinline__ Chunk<T, V> load_chunk(const T* p, int n, bool vec) {
-  Chunk<T, V> c;
-  if (vec && n >= V) {
-    c = *reinterpret_cast<const Chunk<T, V>*>(p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) c.v[i] = i < n ? p[i] : from_f<T>(0.f);
-  }
-  return c;
-}
+// Elements [0, n) of a chunk, as one access where `vec` (the caller has checked alignment) and all are meant.
 template <typename T, int V>
 __device__ __forceinline__ void store_chunk(T* p, const Chunk<T, V>& c, int n, bool vec) {
   if (vec && n >= V) {
@@ -61,7 +50,7 @@ __device__ __forceinline__ void store_chunk(T* p, const Chunk<T, V>& c, int n, b
 }
 
 // All V elements or none (zeros): one predicated access, so that the loads of a loop's next turn can stay in flight
-// (a choice between paths, as above, makes the thread wait for the values where the paths meet).
+// (a choice between two ways to load makes the thread wait for the values where the ways meet).
 template <typename T, int V>
 __device__ __forceinline__ Chunk<T, V> load_whole(const T* p, bool on) {
   Chunk<T, V> c{};

@@ -13,10 +13,9 @@
 // each step asks for bound it: they go through reduce_scatter over the lanes, dB and dC then through
 // shared memory over the block's warps and through a partial array over the channel tiles.
 //
-// Measured on B200, 4 x 2048 x 4096 with 16 states in bf16: 1020 us and 17 us for the sums over the channel tiles
+// Measured on B200, 4 x 2048 x 4096 with 16 states in bf16: 983 us and 17 us for the sums over the channel tiles
 // (29 instructions per (position, channel, state) before the series near 1 was added, schedulers 50 % busy at two
-// warps each: the 16 states of a tile take 128 registers).  One channel per lane, or two states, halve those and
-// double the warps, but need more instructions for each: 1125 and 1046 us against 886 us then.
+// warps each: the 16 states of a tile take 128 registers).
 #include <algorithm>
 
 #include "bst_scan.cuh"
@@ -317,14 +316,33 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
     __syncthreads();
 
     {
-      float2 x[TURNS], y[TURNS], g[TURNS], slope[TURNS];
+      float2 x[TURNS], v[TURNS], slope[TURNS];
+      // Values of this thread's positions, to be stored behind `to`: branches stand outside of the loops.
+      const bool inside = a.vec && in1 && rows == kScanTile;
+      auto put = [&](T* to) {
+        T* p = to + (t0 + row0) * a.channels;
+        const int64_t step = int64_t(ROWS) * a.channels;
+        if (inside) {
+#pragma unroll
+          for (int i = 0; i < TURNS; ++i) *reinterpret_cast<Chunk<T, 2>*>(p + i * step) = to_pair<T>(v[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < TURNS; ++i)
+            if (t0 + row0 + i * ROWS < a.length)
+              store_chunk<T, 2>(p + i * step, to_pair<T>(v[i]), left - col, false);
+        }
+      };
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int r = row0 + i * ROWS;
+        const float2 e = *reinterpret_cast<const float2*>(&m.e[r][col]);
         x[i] = load_pair(&act[0][r][col]);
-        g[i] = *reinterpret_cast<const float2*>(&m.sum_g[r][col]);
+        dD = fma2(e, x[i], dD);
+        v[i] = fma2(*reinterpret_cast<const float2*>(&m.d[r][col]), *reinterpret_cast<const float2*>(&m.sum_g[r][col]),
+                    mul2(skip, e));
         slope[i] = both(1.f);
       }
+      put(du);
       if (a.softplus) {
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) slope[i] = sigmoid2(add2(load_pair(&act[1][row0 + i * ROWS][col]), bias));
@@ -332,32 +350,23 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int r = row0 + i * ROWS;
-        const int64_t t = t0 + r;
         const float2 w = *reinterpret_cast<const float2*>(&m.sum_w[r][col]);
-        const float2 e = *reinterpret_cast<const float2*>(&m.e[r][col]);
-        const float2 d = *reinterpret_cast<const float2*>(&m.d[r][col]);
-        const float2 dd = r < rows ? mul2(slope[i], fma2(w, both(kLn2), mul2(g[i], x[i]))) : both(0.f);
-        dD = fma2(e, x[i], dD);
-        dbias = make_float2(dbias.x + dd.x, dbias.y + dd.y);
-        if (t < a.length) {
-          store_chunk<T, 2>(du + t * a.channels, to_pair<T>(fma2(d, g[i], mul2(skip, e))), left - col, a.vec);
-          store_chunk<T, 2>(ddl + t * a.channels, to_pair<T>(dd), left - col, a.vec);
-        }
+        const float2 dd = mul2(slope[i], fma2(w, both(kLn2), mul2(*reinterpret_cast<const float2*>(&m.sum_g[r][col]),
+                                                                  x[i])));
+        v[i] = r < rows ? dd : both(0.f);
+        dbias = add2(dbias, v[i]);
       }
+      put(ddl);
       if (a.z) {
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
           const int r = row0 + i * ROWS;
           const float2 z = load_pair(&act[3][r][col]), s = sigmoid2(z);
-          y[i] = fma2(skip, x[i], *reinterpret_cast<const float2*>(&m.sum_y[r][col]));
+          const float2 y = fma2(skip, x[i], *reinterpret_cast<const float2*>(&m.sum_y[r][col]));
           const float2 q = mul2(s, fma2(z, make_float2(1.f - s.x, 1.f - s.y), both(1.f)));
-          y[i] = r < rows ? mul2(mul2(load_pair(&act[2][r][col]), y[i]), q) : both(0.f);
+          v[i] = r < rows ? mul2(mul2(load_pair(&act[2][r][col]), y), q) : both(0.f);
         }
-#pragma unroll
-        for (int i = 0; i < TURNS; ++i) {
-          const int64_t t = t0 + row0 + i * ROWS;
-          if (t < a.length) store_chunk<T, 2>(dz + t * a.channels, to_pair<T>(y[i]), left - col, a.vec);
-        }
+        put(dz);
       }
     }
     for (int j = threadIdx.x; j < kScanTile * 2 * NP; j += NT) {
@@ -456,14 +465,18 @@ __global__ void __launch_bounds__(256) scan_params_kernel(const ScanArgs a, int 
 }
 
 // ---- host ------------------------------------------------------------------------------
-// The block shape for N states, as f(ScanShape).
+// The block shape of a request, as f(ScanShape).  Two channels per lane need fewer instructions, one channel half of
+// the registers for a tile's states and gives twice the warps, which pays until its blocks (three per SM) no longer
+// fit at once: 384 channel-state pairs per scheduler.  16 states, two | one: 5 x 777 x 514 in fp32 311 | 210 us,
+// 2 x 2048 x 4096 in bf16 930 | 640, 4 x 2048 x 4096, before the series near 1, 886 | 1125.
 template <class F>
-static auto with_backward_shape(int64_t states, F&& f) {
-  switch (scan_pad(states)) {
+static auto with_backward_shape(const bst_scan_desc* d, F&& f) {
+  const int64_t pairs = d->batch * d->channels * scan_pad(d->states) / (int64_t(sm_count()) * 4);
+  switch (scan_pad(d->states)) {
     case 4: return f(ScanShape<2, 2, 2, 2>{});
     case 8: return f(ScanShape<2, 2, 4, 4>{});
-    case 16: return f(ScanShape<4, 2, 4, 4>{});
-    case 32: return f(ScanShape<4, 2, 8, 4>{});
+    case 16: return pairs >= 384 ? f(ScanShape<4, 2, 4, 4>{}) : f(ScanShape<4, 1, 4, 4>{});
+    case 32: return pairs >= 384 ? f(ScanShape<4, 2, 8, 4>{}) : f(ScanShape<4, 1, 8, 4>{});
     default: return f(ScanShape<4, 2, 16, 4>{});
   }
 }
@@ -473,7 +486,7 @@ struct BackwardLayout {
 };
 static BackwardLayout backward_layout(const bst_scan_desc* d) {
   const int64_t np = scan_pad(d->states);
-  const int64_t ct = with_backward_shape(d->states, [](auto sh) { return int64_t(decltype(sh)::CT); });
+  const int64_t ct = with_backward_shape(d, [](auto sh) { return int64_t(decltype(sh)::CT); });
   const int64_t per_group = d->channels / d->groups, tiles = (per_group + ct - 1) / ct;
   BackwardLayout l{};
   l.pa = d->batch * d->groups * tiles * d->length * 2 * np * 4;
@@ -550,7 +563,7 @@ extern "C" int bst_scan_backward(const bst_scan_desc* d, const void* u, const vo
   if (!a.error) return fail(BST_ERR_CUDA, "device error word unavailable");
   int rc = with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
-    return with_backward_shape(d->states, [&](auto sh) { return scan_backward_launch<T, decltype(sh)>(d, a, st); });
+    return with_backward_shape(d, [&](auto sh) { return scan_backward_launch<T, decltype(sh)>(d, a, st); });
   });
   if (rc) return rc;
   const int np = scan_pad(d->states);
