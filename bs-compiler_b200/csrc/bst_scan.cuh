@@ -140,17 +140,29 @@ struct alignas(4 * S) Pairs {
 // one is `me`, in words or elements.  The other columns are filled with zeros, the other rows left as they were.
 template <typename T, int WIDTH, int NT>
 __device__ __forceinline__ void stage_tile(T* to, const T* from, int64_t step, int rows, int cols, bool words, int me) {
-  constexpr int P = 4 / int(sizeof(T)), ACROSS = WIDTH / P;
   if (words) {
-    for (int k = me; k < rows * ACROSS; k += NT) {
-      const int r = k / ACROSS, c = k % ACROSS * P;
-      if (c < cols) copy_async4(to + r * WIDTH + c, from + r * step + c);
-      else *reinterpret_cast<uint32_t*>(to + r * WIDTH + c) = 0;
+    constexpr int P = 4 / int(sizeof(T)), ACROSS = WIDTH / P, ITEMS = kScanTile * ACROSS;
+#pragma unroll
+    for (int i = 0; i < (ITEMS + NT - 1) / NT; ++i) {
+      const int k = me + i * NT, r = k / ACROSS, c = k % ACROSS * P;
+      if (r < rows) {
+        if (c < cols) copy_async4(to + r * WIDTH + c, from + r * step + c);
+        else *reinterpret_cast<uint32_t*>(to + r * WIDTH + c) = 0;
+      }
     }
   } else {
-    for (int k = me; k < rows * WIDTH; k += NT) {
-      const int r = k / WIDTH, c = k % WIDTH;
-      to[k] = c < cols ? from[r * step + c] : from_f<T>(0.f);
+    constexpr int ITEMS = kScanTile * WIDTH, N = (ITEMS + NT - 1) / NT;
+    T v[N];  // all loads before the first store
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int k = me + i * NT, r = k / WIDTH, c = k % WIDTH;
+      v[i] = from_f<T>(0.f);
+      if (r < rows && c < cols) v[i] = from[r * step + c];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int k = me + i * NT;
+      if (k / WIDTH < rows) to[k] = v[i];
     }
   }
 }

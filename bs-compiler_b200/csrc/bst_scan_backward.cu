@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(Sh::NT) scan_backward_kernel(const ScanArgs a,
           }
         for (int j = rows * NP + int(threadIdx.x); j < kScanTile * NP; j += NT)
           (&m.bc[slot][0][0][0])[j] = (&m.bc[slot][1][0][0])[j] = from_f<T>(0.f);
+        if constexpr (TILES) fence_proxy_async_smem();  // before the copy engine writes to this slot again
       }
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
