@@ -84,7 +84,7 @@ def conv_channels_first(x, weight, bias, activation):
 
 
 def _causal_conv(n):
-    """(last node of the pattern, x, weight, bias) of a causal depthwise convolution at conv1d node n."""
+    """(nodes of the pattern, x, weight, bias) of a causal depthwise convolution at conv1d node n."""
     x, w, b = _arg(n, 0, "input"), _arg(n, 1, "weight"), _arg(n, 2, "bias")
     stride, pad = _arg(n, 3, "stride", 1), _arg(n, 4, "padding", 0)
     dilation, groups = _arg(n, 5, "dilation", 1), _arg(n, 6, "groups", 1)
@@ -102,10 +102,10 @@ def _causal_conv(n):
         src = _value(_arg(x, 0, "input"))
         if (src is not None and spec == (taps - 1, 0) and _arg(x, 2, "mode", "constant") == "constant"
                 and _arg(x, 3, "value") in (None, 0, 0.0)):
-            return n, _arg(x, 0, "input"), w, b
+            return [x, n], _arg(x, 0, "input"), w, b
         return None
     if taps == 1 and _one(pad, 0):
-        return n, x, w, b
+        return [n], x, w, b
     if not _one(pad, taps - 1) or len(n.users) != 1:
         return None
     cut = next(iter(n.users))
@@ -121,14 +121,20 @@ def _causal_conv(n):
         return None
     if last.stop != length and not (taps > 1 and last.stop == 1 - taps):
         return None
-    return cut, x, w, b
+    return [n, cut], x, w, b
 
 
-def _replace(gm, node, fn, args):
-    with gm.graph.inserting_before(node):
+def _replace(gm, nodes, fn, args):
+    """fn(*args) in place of the last of a pattern's nodes (in the graph's order).  Those that nothing else reads are
+    erased, and no others: Dynamo's graphs hold the user's in-place operations as nodes without users."""
+    last = nodes[-1]
+    with gm.graph.inserting_before(last):
         new = gm.graph.call_function(fn, args)
-    new.meta = dict(node.meta)
-    node.replace_all_uses_with(new)
+    new.meta = dict(last.meta)
+    last.replace_all_uses_with(new)
+    for n in reversed(nodes):
+        if not n.users:
+            gm.graph.erase_node(n)
 
 
 def has_layer_ops(gm: torch.fx.GraphModule) -> bool:
@@ -145,21 +151,20 @@ def route(gm: torch.fx.GraphModule) -> int:
         if n.target is F.layer_norm:
             hit = _layer_norm(n)
             if hit:
-                _replace(gm, n, *hit)
+                _replace(gm, [n], *hit)
                 count += 1
         elif n.target in _CONV:
             hit = _causal_conv(n)
             if hit:
-                last, x, w, b = hit
+                nodes, x, w, b = hit
                 act = None
-                if len(last.users) == 1:
-                    user = next(iter(last.users))
+                if len(nodes[-1].users) == 1:
+                    user = next(iter(nodes[-1].users))
                     if user.op == "call_function" and user.target in _SILU and not user.kwargs.get("inplace") and \
                             len(user.args) == 1:
-                        last, act = user, "silu"
-                _replace(gm, last, conv_channels_first, (x, w, b, act))
+                        nodes, act = [*nodes, user], "silu"
+                _replace(gm, nodes, conv_channels_first, (x, w, b, act))
                 count += 1
     if count:
-        gm.graph.eliminate_dead_code()
         gm.recompile()
     return count
