@@ -83,6 +83,14 @@ def conv_channels_first(x, weight, bias, activation):
     return layers.causal_conv(x.transpose(1, 2), weight.squeeze(1), bias, activation).transpose(1, 2)
 
 
+def _pad_stays(pad, conv, src):
+    """Whether the convolution may read the source of an F.pad instead of its copy: nothing can write to either before
+    it does, nor to the source behind it (the gradients read it again)."""
+    nodes = list(pad.graph.nodes)
+    i, j = nodes.index(pad), nodes.index(conv)
+    return all(map(_reads_only, nodes[i + 1:j])) and not any(_writes_to(m, src) for m in nodes[j + 1:])
+
+
 def _causal_conv(n):
     """(nodes of the pattern, x, weight, bias) of a causal depthwise convolution at conv1d node n."""
     x, w, b = _arg(n, 0, "input"), _arg(n, 1, "weight"), _arg(n, 2, "bias")
@@ -101,7 +109,7 @@ def _causal_conv(n):
         spec = tuple(_arg(x, 1, "pad"))
         src = _value(_arg(x, 0, "input"))
         if (src is not None and spec == (taps - 1, 0) and _arg(x, 2, "mode", "constant") == "constant"
-                and _arg(x, 3, "value") in (None, 0, 0.0)):
+                and _arg(x, 3, "value") in (None, 0, 0.0) and _pad_stays(x, n, src)):
             return [x, n], _arg(x, 0, "input"), w, b
         return None
     if taps == 1 and _one(pad, 0):
@@ -124,11 +132,46 @@ def _causal_conv(n):
     return [n, cut], x, w, b
 
 
-def _replace(gm, nodes, fn, args):
-    """fn(*args) in place of the last of a pattern's nodes (in the graph's order).  Those that nothing else reads are
-    erased, and no others: Dynamo's graphs hold the user's in-place operations as nodes without users."""
+# What may stand between a pattern's F.pad and its convolution: operations that write to nothing.
+_VIEWS = {"chunk", "contiguous", "detach", "expand", "permute", "reshape", "size", "split", "squeeze", "to", "transpose",
+          "unsqueeze", "view"}
+_READERS = {operator.getitem, F.layer_norm, layers.layer_norm, conv_channels_first} | _PAD | _CONV
+
+
+def _reads_only(n):
+    return n.op in ("placeholder", "get_attr") or n.target in (_VIEWS if n.op == "call_method" else _READERS)
+
+
+def _writes_to(n, value):
+    """Whether a node may write in place to the memory of `value`: an operation that is named or asked to write in
+    place, or one that is not torch's own, with an argument in that memory."""
+    name = n.target if isinstance(n.target, str) else getattr(n.target, "__name__", "")
+    module = getattr(n.target, "__module__", None) or ""
+    if n.op == "output" or _reads_only(n):
+        return False
+    if n.op == "call_method":
+        writes = name.endswith("_") and (not name.endswith("__") or name.startswith(("__i", "__set")))
+    elif isinstance(n.target, torch._ops.OpOverload):
+        writes = n.target._schema.is_mutable
+    elif module in ("_operator", "operator"):
+        writes = name in ("setitem", "delitem") or hasattr(operator, f"__{name}__") and name[0] == "i" and \
+            hasattr(operator, name[1:].rstrip("_"))
+    else:
+        writes = name.endswith("_") or n.op != "call_function" or not (module.startswith("torch") or
+                                                                       hasattr(torch, name))
+    if not (writes or n.kwargs.get("out") is not None or n.kwargs.get("inplace") or any(a is True for a in n.args[1:])):
+        return False
+    memory = value.untyped_storage()._cdata
+    return any(isinstance(v, torch.Tensor) and v.layout is torch.strided and v.untyped_storage()._cdata == memory
+               for v in (a.meta.get("example_value") for a in n.all_input_nodes))
+
+
+def _replace(gm, nodes, at, fn, args):
+    """fn(*args) in place of the last of a pattern's nodes (in the graph's order).  It stands where node `at` read the
+    inputs: what later nodes write to them does not reach it.  Nodes that nothing else reads are erased, and no
+    others: Dynamo's graphs hold the user's in-place operations as nodes without users."""
     last = nodes[-1]
-    with gm.graph.inserting_before(last):
+    with gm.graph.inserting_before(at):
         new = gm.graph.call_function(fn, args)
     new.meta = dict(last.meta)
     last.replace_all_uses_with(new)
@@ -151,7 +194,7 @@ def route(gm: torch.fx.GraphModule) -> int:
         if n.target is F.layer_norm:
             hit = _layer_norm(n)
             if hit:
-                _replace(gm, [n], *hit)
+                _replace(gm, [n], n, *hit)
                 count += 1
         elif n.target in _CONV:
             hit = _causal_conv(n)
@@ -163,7 +206,7 @@ def route(gm: torch.fx.GraphModule) -> int:
                     if user.op == "call_function" and user.target in _SILU and not user.kwargs.get("inplace") and \
                             len(user.args) == 1:
                         nodes, act = [*nodes, user], "silu"
-                _replace(gm, nodes, conv_channels_first, (x, w, b, act))
+                _replace(gm, nodes, n, conv_channels_first, (x, w, b, act))
                 count += 1
     if count:
         gm.recompile()

@@ -87,3 +87,95 @@ def test_replaced_nodes_leave_and_shared_ones_stay(plain):
     gm = same_effects(shared, 1, x=x_(), w=torch.randn(C, 1, TAPS))
     t = targets(gm)
     assert torch.conv1d not in t and F.silu not in t and sum(f in fx_layers._PAD for f in t) == 1
+
+
+def test_later_writes_do_not_reach_a_replaced_node(plain):
+    w = torch.randn(C, 1, TAPS)
+    b = torch.randn(C)
+
+    def input_before_silu(x, w):
+        v = F.conv1d(x, w, padding=TAPS - 1, groups=C)[..., :L]
+        x = x.mul_(2)
+        return F.silu(v) + x
+
+    def weight_before_cut(x, w, b):
+        v = F.conv1d(x, w, b, padding=TAPS - 1, groups=C)
+        w.mul_(3)
+        b.add_(1)
+        return F.silu(v[..., :L])
+
+    def input_behind_norm(x):
+        y = F.layer_norm(x, (L,))
+        x.add_(1)
+        return y
+
+    same_effects(input_before_silu, 1, x=x_(), w=w)
+    same_effects(weight_before_cut, 1, x=x_(), w=w, b=b)
+    same_effects(input_behind_norm, 1, x=x_())
+
+
+def test_a_pad_is_not_read_through_when_something_writes_in_between(plain):
+    w = torch.randn(C, 1, TAPS)
+
+    def source(x, w):
+        p = F.pad(x, (TAPS - 1, 0))
+        x.mul_(2)
+        return F.conv1d(p, w, groups=C)
+
+    def padded(x, w):
+        p = F.pad(x, (TAPS - 1, 0))
+        p[..., 0] = 1.0
+        return F.conv1d(p, w, groups=C)
+
+    def view_of_padded(x, w):
+        p = F.pad(x, (TAPS - 1, 0))
+        torch.relu_(p[..., 2:])
+        return F.conv1d(p, w, groups=C)
+
+    for fn in (source, padded, view_of_padded):
+        same_effects(fn, 0, x=x_(), w=w)
+
+
+def test_several_convolutions_of_one_input(plain):
+    def two(x, w):
+        p, q = F.pad(x, (TAPS - 1, 0)), F.pad(x, (TAPS - 1, 0))
+        return F.conv1d(p, w, groups=C), F.silu(F.conv1d(q, w, groups=C)), F.layer_norm(x, (L,))
+
+    same_effects(two, 3, x=x_(), w=torch.randn(C, 1, TAPS))
+
+
+@pytest.mark.parametrize("write", [lambda x: x.mul_(2), lambda x: F.relu(x, inplace=True), lambda x: F.relu(x, True),
+                                   lambda x: torch.add(x, 1, out=x), lambda x: x[0].zero_(), lambda x: torch.relu_(x),
+                                   lambda x: x.__setitem__(0, 1.0), lambda x: x.__iadd__(1),
+                                   lambda x: torch.ops.aten.mul_.Tensor(x, x)])
+def test_a_pad_whose_source_is_written_later_stays_for_the_gradients(write):
+    """The kernel keeps the source for its gradients, the padded convolution its copy."""
+    w = torch.randn(C, 1, TAPS)
+
+    def fn(x, w):
+        y = F.conv1d(F.pad(x, (TAPS - 1, 0)), w, groups=C)
+        write(x)
+        return y
+
+    def pure(x, w):
+        y = F.conv1d(F.pad(x, (TAPS - 1, 0)), w, groups=C)
+        return y.add_(1), x + 1, F.relu(x), x.mean()
+
+    assert fx_layers.route(as_cuda_sharing(graph_of(fn, x_(), w))) == 0
+    assert fx_layers.route(as_cuda_sharing(graph_of(pure, x_(), w))) == 1
+
+
+def as_cuda_sharing(gm):
+    """As as_cuda, with views of one tensor still in one memory."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    memory = {}
+    with FakeTensorMode():
+        for n in gm.graph.nodes:
+            v = n.meta.get("example_value")
+            if isinstance(v, torch.Tensor):
+                key = v.untyped_storage()._cdata
+                if key not in memory:
+                    room = v.untyped_storage().nbytes() // v.element_size()
+                    memory[key] = torch.empty(room, dtype=v.dtype, device="cuda")
+                n.meta["example_value"] = memory[key].as_strided(v.shape, v.stride(), v.storage_offset())
+    return gm
