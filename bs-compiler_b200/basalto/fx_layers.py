@@ -29,7 +29,9 @@ _CONV = {F.conv1d, torch.conv1d}
 def _value(n):
     """The example tensor of a node, if its sizes are plain numbers."""
     v = n.meta.get("example_value") if isinstance(n, torch.fx.Node) else None
-    if not isinstance(v, torch.Tensor) or any(not isinstance(s, int) for s in (*v.shape, *v.stride())):
+    if not isinstance(v, torch.Tensor) or v.layout is not torch.strided or v.is_nested:
+        return None
+    if any(not isinstance(s, int) for s in (*v.shape, *v.stride())):
         return None
     return v
 
@@ -60,10 +62,10 @@ def _layer_norm(n):
     w, b, eps = _arg(n, 2, "weight"), _arg(n, 3, "bias"), _arg(n, 4, "eps", 1e-5)
     if x is None or not _usable(x) or not isinstance(eps, (int, float)):
         return None
-    shape = (shape,) if isinstance(shape, int) else tuple(shape)
-    if not _keeps_type(n, x):
+    shape = (shape,) if isinstance(shape, int) else shape
+    if not isinstance(shape, (tuple, list)) or not _keeps_type(n, x):
         return None
-    if x.dim() < 1 or shape != (x.shape[-1],) or not (_param_ok(w, x) and _param_ok(b, x) and _same_type(w, b)):
+    if x.dim() < 1 or tuple(shape) != (x.shape[-1],) or not (_param_ok(w, x) and _param_ok(b, x) and _same_type(w, b)):
         return None
     return layers.layer_norm, (_arg(n, 0, "input"), w, b, float(eps))
 
@@ -106,10 +108,11 @@ def _causal_conv(n):
     if not (_param_ok(w, xv) and _param_ok(b, xv) and _same_type(w, b) and _keeps_type(n, xv)):
         return None
     if _one(pad, 0) and isinstance(x, torch.fx.Node) and x.target in _PAD and x.op == "call_function":
-        spec = tuple(_arg(x, 1, "pad"))
+        spec = _arg(x, 1, "pad")
         src = _value(_arg(x, 0, "input"))
-        if (src is not None and spec == (taps - 1, 0) and _arg(x, 2, "mode", "constant") == "constant"
-                and _arg(x, 3, "value") in (None, 0, 0.0) and _pad_stays(x, n, src)):
+        zeros = _arg(x, 2, "mode", "constant") == "constant" and _arg(x, 3, "value") in (None, 0, 0.0)
+        if (src is not None and zeros and isinstance(spec, (tuple, list)) and tuple(spec) == (taps - 1, 0)
+                and _pad_stays(x, n, src)):
             return [x, n], _arg(x, 0, "input"), w, b
         return None
     if taps == 1 and _one(pad, 0):
@@ -120,9 +123,11 @@ def _causal_conv(n):
     if cut.op != "call_function" or cut.target is not operator.getitem:
         return None
     idx = cut.args[1]
-    lead, last = (idx[:-1], idx[-1]) if isinstance(idx, tuple) else ((), None)
-    whole = all(i is Ellipsis or i == slice(None, None, None) for i in lead)
-    if not whole or (len(idx) != 3 and not (len(idx) == 2 and lead[0] is Ellipsis)):
+    if not isinstance(idx, tuple) or len(idx) not in (2, 3):
+        return None
+    lead, last = idx[:-1], idx[-1]
+    whole = all(i is Ellipsis or (isinstance(i, slice) and i == slice(None, None, None)) for i in lead)
+    if not whole or (len(idx) == 2 and lead[0] is not Ellipsis):
         return None
     length = xv.shape[2]
     if not isinstance(last, slice) or last.start not in (None, 0) or last.step not in (None, 1):

@@ -179,3 +179,28 @@ def as_cuda_sharing(gm):
                     memory[key] = torch.empty(room, dtype=v.dtype, device="cuda")
                 n.meta["example_value"] = memory[key].as_strided(v.shape, v.stride(), v.storage_offset())
     return gm
+
+
+def test_other_forms_are_left_alone_without_an_error(plain):
+    """Cuts by something else than a tuple, pads by other ways, inputs without strides."""
+    w = torch.randn(C, 1, TAPS)
+
+    def conv(x, w):
+        return F.conv1d(x, w, padding=TAPS - 1, groups=C)
+
+    cuts = [0, slice(0, L), None, Ellipsis, (Ellipsis,), (), [0, 1], (slice(None), slice(None)),
+            (0, Ellipsis, slice(0, L))]
+    for idx in cuts:
+        same_effects(lambda x, w: conv(x, w)[idx], 0, x=x_(), w=w)
+    same_effects(lambda x, w, i: conv(x, w)[i], 0, x=x_(), w=w, i=torch.tensor([1, 0]))
+    same_effects(lambda x, w: F.conv1d(F.pad(x, (TAPS - 1, 0), "circular"), w, groups=C), 0, x=x_(), w=w)
+    same_effects(lambda x, w: F.conv1d(F.pad(x, [TAPS - 1, 0, 0, 0]), w, groups=C), 0, x=x_(), w=w)
+
+    gm = as_cuda(graph_of(lambda x: F.layer_norm(F.pad(x, (1, 0)), (L + 1,)), x_()))
+    norm, pad = (next(n for n in gm.graph.nodes if n.target in t) for t in ({F.layer_norm}, fx_layers._PAD))
+    norm.update_arg(1, pad)  # a size that the graph computes
+    assert fx_layers.route(gm) == 0
+    gm = as_cuda(graph_of(lambda x: F.layer_norm(x, (L,)), x_()))
+    source = next(n for n in gm.graph.nodes if n.op == "placeholder")
+    source.meta["example_value"] = torch.zeros(2, 3).to_sparse()
+    assert fx_layers.route(gm) == 0
