@@ -80,9 +80,15 @@ def _one(v, want):
     return v == want or (isinstance(v, (tuple, list)) and len(v) == 1 and v[0] == want)
 
 
-def conv_channels_first(x, weight, bias, activation):
-    """causal_conv of x [batch, channels, length] with conv1d's weight [channels, 1, taps]."""
-    return layers.causal_conv(x.transpose(1, 2), weight.squeeze(1), bias, activation).transpose(1, 2)
+def conv_channels_first(x, weight, bias, activation, strides):
+    """causal_conv of x [batch, channels, length] with conv1d's weight [channels, 1, taps], its result in the strides
+    that the graph's code was traced with."""
+    args = x.transpose(1, 2), weight.squeeze(1), bias, activation
+    b, c, n = strides
+    if c == 1 or n == 1:
+        return layers._causal_conv_in((b, n, c), *args).transpose(1, 2)
+    y = layers.causal_conv(*args).transpose(1, 2)
+    return torch.empty_strided(y.shape, strides, dtype=y.dtype, device=y.device).copy_(y)
 
 
 def _pad_stays(pad, conv, src):
@@ -211,7 +217,9 @@ def route(gm: torch.fx.GraphModule) -> int:
                     if user.op == "call_function" and user.target in _SILU and not user.kwargs.get("inplace") and \
                             len(user.args) == 1:
                         nodes, act = [*nodes, user], "silu"
-                _replace(gm, nodes, n, conv_channels_first, (x, w, b, act))
+                if _value(nodes[-1]) is None:
+                    continue
+                _replace(gm, nodes, n, conv_channels_first, (x, w, b, act, tuple(_value(nodes[-1]).stride())))
                 count += 1
     if count:
         gm.recompile()

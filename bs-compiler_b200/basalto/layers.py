@@ -216,15 +216,21 @@ def _lines(x):
 
 def _conv_layout(x, lines=None):
     """(x or a copy of it, lines) in a layout that the kernels take: the given one, or x's own."""
-    own = _lines(x)
-    if own is None or (lines is not None and own != lines):
-        x = x.transpose(1, 2).contiguous().transpose(1, 2) if lines else x.contiguous()
-        own = lines or 0
-    return x, own
+    if lines is None:
+        lines = _lines(x)
+        if lines is not None:
+            return x, lines
+    else:
+        axis = 1 if lines else 2
+        if x.stride(axis) == 1 or x.shape[axis] <= 1:
+            return x, lines
+    return (x.transpose(1, 2).contiguous().transpose(1, 2), 1) if lines else (x.contiguous(), 0)
 
 
-def _conv_empty(x, lines):
+def _conv_empty(x, lines, strides=None):
     b, n, c = x.shape
+    if strides is not None:
+        return torch.empty_strided((b, n, c), strides, dtype=x.dtype, device=x.device)
     if lines:
         return torch.empty(b, c, n, dtype=x.dtype, device=x.device).transpose(1, 2)
     return torch.empty(b, n, c, dtype=x.dtype, device=x.device)
@@ -234,9 +240,10 @@ def _step_of(x, lines):
     return x.stride(2) if lines else x.stride(1)
 
 
-def _conv_forward(x, weight, bias, silu, initial, lengths, want_state):
-    x, lines = _conv_layout(x)
-    y = _conv_empty(x, lines)
+def _conv_forward(x, weight, bias, silu, initial, lengths, want_state, strides=None):
+    """strides: of y, with either axis contiguous (None: x's layout)."""
+    x, lines = _conv_layout(x, None if strides is None else int(strides[2] != 1))
+    y = _conv_empty(x, lines, strides)
     b, n, c = x.shape
     width = weight.shape[1]
     final = torch.empty(b, width - 1, c, dtype=x.dtype, device=x.device) if want_state else None
@@ -276,8 +283,8 @@ def _conv_backward(dy, dfinal, x, weight, bias, silu, initial, lengths, want_bia
 
 class _Conv(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, silu, initial, lengths, want_state):
-        y, final = _conv_forward(x, weight, bias, silu, initial, lengths, want_state)
+    def forward(ctx, x, weight, bias, silu, initial, lengths, want_state, strides):
+        y, final = _conv_forward(x, weight, bias, silu, initial, lengths, want_state, strides)
         ctx.save_for_backward(x, weight, bias, initial, lengths)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -291,7 +298,7 @@ class _Conv(torch.autograd.Function):
             dy = torch.zeros_like(x)
         need = ctx.needs_input_grad
         dx, dw, db, dinit = _conv_backward(dy, dfinal, x, weight, bias, ctx.silu, initial, lengths, need[2], need[4])
-        return dx, dw, db, None, dinit, None, None
+        return dx, dw, db, None, dinit, None, None, None
 
 
 def _conv_args(name, x, weight, bias, activation):
@@ -340,9 +347,20 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, lengt
     if initial_state is not None:
         initial_state = initial_state.contiguous()
     if _wants_grad(x, weight, bias, initial_state):
-        return _Conv.apply(x, weight, bias, silu, initial_state, lengths, bool(return_state))
+        return _Conv.apply(x, weight, bias, silu, initial_state, lengths, bool(return_state), None)
     y, final = _conv_forward(x, weight, bias, silu, initial_state, lengths, return_state)
     return (y, final) if return_state else y
+
+
+def _causal_conv_in(strides, x, weight, bias, activation):
+    """causal_conv whose y has these strides (either its channels or its positions are 1 apart)."""
+    _type("causal_conv", x)
+    silu = _conv_args("causal_conv", x, weight, bias, activation)
+    _cuda("causal_conv", x)
+    weight, bias = weight.contiguous(), _dense(bias)
+    if _wants_grad(x, weight, bias):
+        return _Conv.apply(x, weight, bias, silu, None, None, False, strides)
+    return _conv_forward(x, weight, bias, silu, None, None, False, strides)[0]
 
 
 def _no_grad_step(name, *ts):

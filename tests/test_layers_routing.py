@@ -6,16 +6,23 @@ import pytest
 import torch
 import torch.nn.functional as F
 
+import basalto
 from basalto import fx_layers, layers
 from test_layers_compile import as_cuda, graph_of, targets
 
 C, L, TAPS = 6, 11, 4
 
 
-def plain_conv(x, weight, bias=None, activation=None, **_):
+def plain_conv(x, weight, bias=None, activation=None):
+    """As the kernel: the result has its input's layout."""
     y = F.conv1d(x.transpose(1, 2), weight[:, None], bias, padding=weight.shape[1] - 1, groups=x.shape[2])
     y = y[..., :x.shape[1]].transpose(1, 2)
-    return F.silu(y) if activation else y
+    return torch.empty_like(x).copy_(F.silu(y) if activation else y)
+
+
+def plain_conv_in(strides, *args):
+    y = plain_conv(*args)
+    return torch.empty_strided(y.shape, strides).copy_(y)
 
 
 def plain_norm(x, weight=None, bias=None, eps=1e-5):
@@ -25,6 +32,7 @@ def plain_norm(x, weight=None, bias=None, eps=1e-5):
 @pytest.fixture
 def plain(monkeypatch):
     monkeypatch.setattr(layers, "causal_conv", plain_conv)
+    monkeypatch.setattr(layers, "_causal_conv_in", plain_conv_in, raising=False)
     monkeypatch.setattr(layers, "layer_norm", plain_norm)
 
 
@@ -204,3 +212,72 @@ def test_other_forms_are_left_alone_without_an_error(plain):
     source = next(n for n in gm.graph.nodes if n.op == "placeholder")
     source.meta["example_value"] = torch.zeros(2, 3).to_sparse()
     assert fx_layers.route(gm) == 0
+
+
+def test_results_have_the_layout_that_the_graph_was_traced_with(plain):
+    """A convolution answers with the sequence axis contiguous whatever its input's layout, a cut of it with the
+    padded length between the rows: code behind it may have been traced for that (views, strides)."""
+    w = torch.randn(C, 1, TAPS)
+
+    def padded(x, w):
+        return F.conv1d(F.pad(x, (TAPS - 1, 0)), w, groups=C)
+
+    def cut(x, w):
+        return F.conv1d(x, w, padding=TAPS - 1, groups=C)[..., :L]
+
+    inputs = {"rows": x_(), "channels": x_(False).transpose(1, 2), "spread": torch.randn(2, C, 2 * L)[..., ::2],
+              "one channel": torch.randn(2, 1, L), "one position": torch.randn(2, C, 1)}
+    for x in inputs.values():
+        c, n = x.shape[1:]
+        wx = w[:c]
+        fns = [lambda x, w: F.conv1d(F.pad(x, (TAPS - 1, 0)), w, groups=c),
+               lambda x, w: F.conv1d(x, w, padding=TAPS - 1, groups=c)[..., :n],
+               lambda x, w: F.silu(F.conv1d(x, w, padding=TAPS - 1, groups=c)[..., :n])]
+        for fn in fns:
+            gm = graph_of(fn, x, wx)
+            want = [m.meta["example_value"].stride() for m in gm.graph.nodes if m.op != "output"][-1]
+            assert fx_layers.route(as_cuda(gm)) == 1
+            got = gm(*[x if m.name == "l_x_" else wx for m in gm.graph.nodes if m.op == "placeholder"])[0]
+            assert got.stride() == want and torch.allclose(got, fn(x, wx), rtol=1e-5, atol=1e-6)
+
+    def viewed(x, w):
+        y = padded(x, w)
+        return y.view(x.shape[0], -1), y.as_strided((2, 3), (C * L, 1))
+
+    same_effects(viewed, 1, x=inputs["channels"], w=w)
+    same_effects(lambda x, w: (cut(x, w).as_strided((2, C), (C * (L + TAPS - 1), L + TAPS - 1)),), 1,
+                 x=inputs["channels"], w=w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["rows", "channels"])
+@pytest.mark.parametrize("form", ["pad", "cut", "silu"])
+def test_compiled_layouts_on_the_kernels(monkeypatch, layout, form):
+    """The same through the backend, with gradients, against conv1d in 64 bits."""
+    monkeypatch.setenv("BASALTO_MODEL_OPS", "1")
+    n = 37
+    x = torch.randn(2, C, n, device="cuda") if layout == "rows" else torch.randn(2, n, C, device="cuda").transpose(1, 2)
+    w = torch.randn(C, 1, TAPS, device="cuda")
+
+    def fn(x, w):
+        if form == "pad":
+            y = F.conv1d(F.pad(x, (TAPS - 1, 0)), w, groups=C)
+            return y.view(x.shape[0], -1)
+        y = F.conv1d(x, w, padding=TAPS - 1, groups=C)[..., :x.shape[2]]
+        return F.silu(y).view(x.shape[0], -1) if form == "silu" else y
+
+    torch._dynamo.reset()
+    cf = torch.compile(fn, backend="basalto", dynamic=False)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    n0 = basalto.launch_count()
+    y = cf(*leaves)
+    assert basalto.launch_count() == n0 + 1
+    if form == "cut":
+        assert y.stride() == (C * (n + TAPS - 1), n + TAPS - 1, 1)
+    exact = [t.detach().double().requires_grad_() for t in leaves]
+    want = fn(*exact)
+    dy = torch.randn_like(want)
+    got = [y, *torch.autograd.grad(y, leaves, dy.float())]
+    # Values and weights to 5, sums over 4 taps, or 74 positions for the weights: 74 * 25 * 8 half steps of 2^-24.
+    for a, b in zip(got, [want, *torch.autograd.grad(want, exact, dy)]):
+        assert (a.double() - b).abs().max() <= 74 * 25 * 8 * 2.0 ** -24
