@@ -24,6 +24,7 @@ _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _SILU = {F.silu, torch.ops.aten.silu.default}
 _PAD = {F.pad, getattr(torch._C._nn, "pad", F.pad)}
 _CONV = {F.conv1d, torch.conv1d}
+_MOST_SEQUENCES = 65535  # of a convolution's launch
 
 
 def _value(n):
@@ -60,7 +61,7 @@ def _layer_norm(n):
     x = _value(_arg(n, 0, "input"))
     shape = _arg(n, 1, "normalized_shape")
     w, b, eps = _arg(n, 2, "weight"), _arg(n, 3, "bias"), _arg(n, 4, "eps", 1e-5)
-    if x is None or not _usable(x) or not isinstance(eps, (int, float)):
+    if x is None or not _usable(x) or not isinstance(eps, (int, float)) or not eps >= 0:
         return None
     shape = (shape,) if isinstance(shape, int) else shape
     if not isinstance(shape, (tuple, list)) or not _keeps_type(n, x):
@@ -106,6 +107,8 @@ def _causal_conv(n):
     dilation, groups = _arg(n, 5, "dilation", 1), _arg(n, 6, "groups", 1)
     xv, wv = _value(x), _value(w)
     if xv is None or wv is None or not _usable(xv, wv) or xv.dim() != 3 or wv.dim() != 3:
+        return None
+    if xv.shape[0] > _MOST_SEQUENCES:
         return None
     c, taps = xv.shape[1], wv.shape[2]
     if groups != c or tuple(wv.shape) != (c, 1, taps) or not 1 <= taps <= 8 or not (_one(stride, 1) and

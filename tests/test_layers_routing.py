@@ -281,3 +281,17 @@ def test_compiled_layouts_on_the_kernels(monkeypatch, layout, form):
     # Values and weights to 5, sums over 4 taps, or 74 positions for the weights: 74 * 25 * 8 half steps of 2^-24.
     for a, b in zip(got, [want, *torch.autograd.grad(want, exact, dy)]):
         assert (a.double() - b).abs().max() <= 74 * 25 * 8 * 2.0 ** -24
+
+
+def test_what_the_kernels_refuse_is_left_alone():
+    """More sequences than a launch can hold, a negative eps: eager torch runs them."""
+    w, meta = torch.randn(C, 1, TAPS), torch.device("meta")
+
+    def conv(x, w):
+        return F.conv1d(x, w, padding=TAPS - 1, groups=C)[..., :2]
+
+    for batch, want in ((65535, 1), (65536, 0)):
+        assert fx_layers.route(as_cuda(graph_of(conv, torch.empty(batch, C, 2, device=meta), w.to(meta)))) == want
+    for eps, want in ((0.0, 1), (-1e-3, 0), (float("nan"), 0)):
+        gm = as_cuda(graph_of(lambda x: F.layer_norm(x, (C,), eps=eps), x_(False)))
+        assert fx_layers.route(gm) == want
