@@ -61,7 +61,7 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool, i
                 lengths: Optional[Tensor]) -> tuple[Tensor, Tensor]:
     L._cuda("causal_conv", x)
     return L._conv_forward(x, weight.contiguous(), L._dense(bias), int(silu),
-                           None if initial is None else initial.contiguous(), lengths, True)
+                           None if initial is None else initial.contiguous(), L._dense(lengths), True)
 
 
 @causal_conv.register_fake
@@ -73,8 +73,8 @@ def _(x, weight, bias, silu, initial, lengths):
 def causal_conv_backward(dy: Tensor, dfinal: Tensor, x: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool,
                          initial: Optional[Tensor], lengths: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     dx, dw, db, dinit = L._conv_backward(dy, dfinal, x, weight.contiguous(), L._dense(bias), int(silu),
-                                         None if initial is None else initial.contiguous(), lengths, bias is not None,
-                                         initial is not None)
+                                         None if initial is None else initial.contiguous(), L._dense(lengths),
+                                         bias is not None, initial is not None)
     return dx, dw, x.new_empty(0) if db is None else db, x.new_empty(0) if dinit is None else dinit
 
 
@@ -107,8 +107,8 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
                    lengths: Optional[Tensor], save: bool) -> tuple[Tensor, Tensor, Tensor]:
     L._cuda("selective_scan", u)
     y, final, saved = L._scan_forward(u, delta, A.contiguous(), B, C, L._dense(D), z, L._dense(delta_bias),
-                                      int(softplus), None if initial is None else initial.contiguous(), lengths, True,
-                                      save)
+                                      int(softplus), None if initial is None else initial.contiguous(),
+                                      L._dense(lengths), True, save)
     return y, final, u.new_empty(0, dtype=torch.uint8) if saved is None else saved
 
 
@@ -125,7 +125,7 @@ def selective_scan_backward(dy: Tensor, dfinal: Tensor, u: Tensor, delta: Tensor
                             D: Optional[Tensor], z: Optional[Tensor], delta_bias: Optional[Tensor], softplus: bool,
                             lengths: Optional[Tensor], saved: Tensor) -> list[Tensor]:
     out = L._scan_backward(dy, dfinal, u, delta, A.contiguous(), B, C, L._dense(D), z, L._dense(delta_bias),
-                           int(softplus), lengths, saved, True)
+                           int(softplus), L._dense(lengths), saved, True)
     return [u.new_empty(0) if t is None else t for t in out]
 
 

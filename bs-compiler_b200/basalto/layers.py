@@ -83,10 +83,8 @@ def _dense(t):
 
 
 def _lengths(name, lengths, batch, device):
-    if lengths is None:
-        return None
-    _need(name, "lengths", lengths, (batch,), torch.int32, device)
-    return lengths.contiguous()
+    if lengths is not None:
+        _need(name, "lengths", lengths, (batch,), torch.int32, device)
 
 
 def _wants_grad(*ts):
@@ -335,7 +333,7 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, lengt
     b, _, c = x.shape
     if initial_state is not None:
         _need(name, "initial_state", initial_state, (b, weight.shape[1] - 1, c), x.dtype, x.device)
-    lengths = _lengths(name, lengths, b, x.device)
+    _lengths(name, lengths, b, x.device)
     if torch.compiler.is_compiling():
         _no_stream(name, stream)
         y, final = torch.ops.basalto.causal_conv(x, weight, bias, bool(silu), initial_state, lengths)
@@ -343,7 +341,7 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, lengt
     _cuda(name, x)
     if stream is not None:
         return _on(stream, causal_conv, x, weight, bias, activation, initial_state, lengths, return_state)
-    weight, bias = weight.contiguous(), _dense(bias)
+    weight, bias, lengths = weight.contiguous(), _dense(bias), _dense(lengths)
     if initial_state is not None:
         initial_state = initial_state.contiguous()
     if _wants_grad(x, weight, bias, initial_state):
@@ -579,7 +577,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     b, _, c = u.shape
     if initial_state is not None:
         _need(name, "initial_state", initial_state, (b, c, A.shape[1]), torch.float32, u.device)
-    lengths = _lengths(name, lengths, b, u.device)
+    _lengths(name, lengths, b, u.device)
     if torch.compiler.is_compiling():
         _no_stream(name, stream)
         save = _wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state)
@@ -591,7 +589,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
         return _on(stream, selective_scan, u, delta, A, B, C, D, z, delta_bias, delta_softplus, initial_state, lengths,
                    return_state)
     softplus = 1 if delta_softplus else 0
-    A, D, delta_bias = A.contiguous(), _dense(D), _dense(delta_bias)
+    A, D, delta_bias, lengths = A.contiguous(), _dense(D), _dense(delta_bias), _dense(lengths)
     if initial_state is not None:
         initial_state = initial_state.contiguous()
     if _wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state):
