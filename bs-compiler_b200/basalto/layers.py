@@ -7,8 +7,8 @@
 
 They run on CUDA tensors in float32, bfloat16 or float16, on the current stream of the tensors' device (or
 on `stream=`: the outputs are then that stream's); arithmetic, statistics and scan states are float32.  The
-first three are differentiable, once.  Under torch.compile they appear in the graph as the custom operators
-torch.ops.basalto.*; the two step functions mutate a state and run outside of compiled graphs.
+first three are differentiable, once, in reverse mode.  Under torch.compile they appear in the graph as the custom
+operators torch.ops.basalto.*; the two step functions mutate a state and run outside of compiled graphs.
 
 Errors: RuntimeError for tensors that are not on one CUDA device and for what the library refuses
 (`_abi.BasaltoError`), TypeError for element types, ValueError for shapes.
@@ -18,6 +18,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _abi, _rust
@@ -95,9 +96,21 @@ def _wants_grad(*ts):
     return False
 
 
-def _no_stream(name, stream):
+def _no_tangents(name, *ts):
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"basalto.{name} has no forward-mode derivative")
+
+
+def _recorded(name, stream, *ts):
+    """Whether this call becomes a custom operator of a compiled graph."""
+    if not torch.compiler.is_compiling():
+        _no_tangents(name, *ts)
+        return False
     if stream is not None:
         raise RuntimeError(f"basalto.{name}: stream= is not available in compiled graphs")
+    return True
 
 
 def _on(stream, fn, *args):
@@ -192,8 +205,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stream=None):
         if p is not None:
             _param(name, what, p, (x.shape[-1],), x)
     _same_params(name, weight, bias)
-    if torch.compiler.is_compiling():
-        _no_stream(name, stream)
+    if _recorded(name, stream, x, weight, bias):
         return torch.ops.basalto.layer_norm(x, weight, bias, eps)[0]
     _cuda(name, x)
     if stream is not None:
@@ -334,8 +346,7 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, lengt
     if initial_state is not None:
         _need(name, "initial_state", initial_state, (b, weight.shape[1] - 1, c), x.dtype, x.device)
     _lengths(name, lengths, b, x.device)
-    if torch.compiler.is_compiling():
-        _no_stream(name, stream)
+    if _recorded(name, stream, x, weight, bias, initial_state):
         y, final = torch.ops.basalto.causal_conv(x, weight, bias, bool(silu), initial_state, lengths)
         return (y, final) if return_state else y
     _cuda(name, x)
@@ -354,6 +365,7 @@ def _causal_conv_in(strides, x, weight, bias, activation):
     """causal_conv whose y has these strides (either its channels or its positions are 1 apart)."""
     _type("causal_conv", x)
     silu = _conv_args("causal_conv", x, weight, bias, activation)
+    _no_tangents("causal_conv", x, weight, bias)
     _cuda("causal_conv", x)
     weight, bias = weight.contiguous(), _dense(bias)
     if _wants_grad(x, weight, bias):
@@ -364,6 +376,7 @@ def _causal_conv_in(strides, x, weight, bias, activation):
 def _no_grad_step(name, *ts):
     if _wants_grad(*ts):
         raise RuntimeError(f"basalto.{name} is not differentiable: call it under torch.no_grad()")
+    _no_tangents(name, *ts)
 
 
 def _out_state(name, state, out_state):
@@ -408,7 +421,6 @@ def causal_conv_step(x, state, weight, bias=None, activation=None, out_state=Non
         return _eager_conv_step(x, state, weight, bias, activation, out_state, stream)
     name = "causal_conv_step"
     code = _type(name, x)
-    _cuda(name, x)
     if x.dim() != 2:
         raise ValueError(f"basalto.causal_conv_step: x must be [batch, channels], got {tuple(x.shape)}")
     silu = _conv_args(name, x, weight, bias, activation)
@@ -416,6 +428,7 @@ def causal_conv_step(x, state, weight, bias=None, activation=None, out_state=Non
     width = weight.shape[1]
     _need(name, "state", state, (b, width - 1, c), x.dtype, x.device)
     _no_grad_step(name, x, state, weight, bias)
+    _cuda(name, x)
     out = _out_state(name, state, out_state)
     if stream is not None:
         return _on(stream, causal_conv_step, x, state, weight, bias, activation, out)
@@ -578,8 +591,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     if initial_state is not None:
         _need(name, "initial_state", initial_state, (b, c, A.shape[1]), torch.float32, u.device)
     _lengths(name, lengths, b, u.device)
-    if torch.compiler.is_compiling():
-        _no_stream(name, stream)
+    if _recorded(name, stream, u, delta, A, B, C, D, z, delta_bias, initial_state):
         save = _wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state)
         y, final, _ = torch.ops.basalto.selective_scan(u, delta, A, B, C, D, z, delta_bias, bool(delta_softplus),
                                                        initial_state, lengths, save)
@@ -610,7 +622,6 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
         return _eager_scan_step(u, delta, A, B, C, state, D, z, delta_bias, delta_softplus, out_state, stream)
     name = "selective_scan_step"
     code = _type(name, u)
-    _cuda(name, u)
     if u.dim() != 2:
         raise ValueError(f"basalto.selective_scan_step: u must be [batch, channels], got {tuple(u.shape)}")
     B, C = _scan_args(name, u, delta, A, B, C, D, z, delta_bias)
@@ -618,6 +629,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     n = A.shape[1]
     _need(name, "state", state, (b, c, n), torch.float32, u.device)
     _no_grad_step(name, u, delta, A, B, C, state, D, z, delta_bias)
+    _cuda(name, u)
     out = _out_state(name, state, out_state)
     if stream is not None:
         return _on(stream, selective_scan_step, u, delta, A, B, C, state, D, z, delta_bias, delta_softplus, out)

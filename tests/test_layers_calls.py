@@ -61,3 +61,32 @@ def test_strided_lengths_in_compiled_graphs():
     grads = [torch.autograd.grad(sum(y.sum() for y in r), x)[0] for r in (got, want)]
     for a, b in zip([*got, grads[0]], [*want, grads[1]]):
         assert torch.equal(a, b)
+
+
+# ---- forward-mode derivatives and traces ----------------------------------------------------------
+def all_calls(x):
+    """Every operator as a function of its first input, x [2, 5, 8]."""
+    c = x.shape[2]
+    w, A, B = parameters(x)
+    conv0, h0 = torch.zeros(2, 3, c, device=x.device), torch.zeros(2, c, 4, device=x.device)
+    return {"layer_norm": lambda x: basalto.layer_norm(x),
+            "causal_conv": lambda x: basalto.causal_conv(x, w),
+            "selective_scan": lambda x: basalto.selective_scan(x, x, A, B, B),
+            "causal_conv_step": lambda x: basalto.causal_conv_step(x[:, 0], conv0, w)[0],
+            "selective_scan_step": lambda x: basalto.selective_scan_step(x[:, 0], x[:, 0], A, B[:, 0], B[:, 0], h0)[0]}
+
+
+@pytest.mark.parametrize("op", sorted(all_calls(torch.zeros(2, 5, 8))))
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_forward_mode_derivatives_are_refused(op, dev):
+    """They would be lost without a word: the result comes from a kernel that knows no tangents."""
+    x = torch.randn(2, 5, 8, device=dev)
+    fn = all_calls(x)[op]
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fn(dual)
+        if dev == "cuda":
+            assert torch.isfinite(fn(x)).all()  # others may run meanwhile
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(fn, (x,), (torch.ones_like(x),))
