@@ -7,8 +7,9 @@
 
 They run on CUDA tensors in float32, bfloat16 or float16, on the current stream of the tensors' device (or
 on `stream=`: the outputs are then that stream's); arithmetic, statistics and scan states are float32.  The
-first three are differentiable, once, in reverse mode.  Under torch.compile they appear in the graph as the custom
-operators torch.ops.basalto.*; the two step functions mutate a state and run outside of compiled graphs.
+first three are differentiable, once, in reverse mode.  Under torch.compile, torch.jit.trace and make_fx they appear
+in the graph as the custom operators torch.ops.basalto.*; the two step functions mutate a state, run outside of
+compiled graphs and refuse to be traced.
 
 Errors: RuntimeError for tensors that are not on one CUDA device and for what the library refuses
 (`_abi.BasaltoError`), TypeError for element types, ValueError for shapes.
@@ -103,13 +104,24 @@ def _no_tangents(name, *ts):
                 raise RuntimeError(f"basalto.{name} has no forward-mode derivative")
 
 
+def _tracing():
+    """Whether torch operators are being recorded (torch.jit.trace, make_fx): a launch would be missing there."""
+    if torch._C._get_tracing_state() is not None:
+        return True
+    if torch._C._len_torch_dispatch_stack() or torch._ops._len_torch_dispatch_stack_pre_dispatch():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        return get_proxy_mode() is not None
+    return False
+
+
 def _recorded(name, stream, *ts):
-    """Whether this call becomes a custom operator of a compiled graph."""
+    """Whether this call becomes a custom operator of a graph: under Dynamo or in a trace."""
     if not torch.compiler.is_compiling():
         _no_tangents(name, *ts)
-        return False
+        if not _tracing():
+            return False
     if stream is not None:
-        raise RuntimeError(f"basalto.{name}: stream= is not available in compiled graphs")
+        raise RuntimeError(f"basalto.{name}: stream= is not available in compiled graphs and traces")
     return True
 
 
@@ -377,6 +389,8 @@ def _no_grad_step(name, *ts):
     if _wants_grad(*ts):
         raise RuntimeError(f"basalto.{name} is not differentiable: call it under torch.no_grad()")
     _no_tangents(name, *ts)
+    if _tracing():
+        raise RuntimeError(f"basalto.{name} writes to its state and cannot be traced")
 
 
 def _out_state(name, state, out_state):
@@ -592,7 +606,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
         _need(name, "initial_state", initial_state, (b, c, A.shape[1]), torch.float32, u.device)
     _lengths(name, lengths, b, u.device)
     if _recorded(name, stream, u, delta, A, B, C, D, z, delta_bias, initial_state):
-        save = _wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state)
+        # Dynamo makes another graph for inputs with gradients; a trace has to serve those too.
+        save = not torch.compiler.is_compiling() or _wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state)
         y, final, _ = torch.ops.basalto.selective_scan(u, delta, A, B, C, D, z, delta_bias, bool(delta_softplus),
                                                        initial_state, lengths, save)
         return (y, final) if return_state else y

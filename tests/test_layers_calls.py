@@ -90,3 +90,42 @@ def test_forward_mode_derivatives_are_refused(op, dev):
             assert torch.isfinite(fn(x)).all()  # others may run meanwhile
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(fn, (x,), (torch.ones_like(x),))
+
+
+def test_a_trace_on_fake_tensors_holds_the_operators():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with FakeTensorMode():
+        x = torch.empty(2, 5, 8, device="cuda")
+        for op, fn in all_calls(x).items():
+            for pre in (False, True):
+                if op.endswith("step"):
+                    with pytest.raises(RuntimeError, match="traced"):
+                        make_fx(fn, pre_dispatch=pre)(x)
+                else:
+                    graph = make_fx(fn, pre_dispatch=pre)(x).graph
+                    assert any(str(n.target) == f"basalto.{op}.default" for n in graph.nodes)
+                    with pytest.raises(RuntimeError, match="stream="):
+                        make_fx(lambda x: basalto.layer_norm(x, stream="another"), pre_dispatch=pre)(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["layer_norm", "causal_conv", "selective_scan"])
+def test_traces_run_the_kernels(op):
+    """torch.jit.trace and make_fx on real tensors, replayed with others; the traced graph has gradients."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, other = torch.randn(2, 5, 8, device="cuda"), torch.randn(2, 5, 8, device="cuda", requires_grad=True)
+    fn = all_calls(x)[op]
+    want = fn(other)
+    grad = torch.autograd.grad(want.sum(), other)[0]
+    for trace in (torch.jit.trace(fn, x), make_fx(fn)(x)):
+        got = trace(other)
+        assert torch.equal(got, want) and torch.equal(torch.autograd.grad(got.sum(), other)[0], grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["causal_conv_step", "selective_scan_step"])
+def test_steps_refuse_traces(op):
+    x = torch.randn(2, 5, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(all_calls(x)[op], x)
