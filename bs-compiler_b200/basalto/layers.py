@@ -21,6 +21,7 @@ import contextlib
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _abi, _rust
 
@@ -459,6 +460,7 @@ def causal_conv_step(x, state, weight, bias=None, activation=None, out_state=Non
                                     out.data_ptr(), out.stride(0), _stream(x))
     if rc:
         _abi.check(rc)
+    increment_version(out)  # autograd's check on saved tensors sees the write
     return y, out
 
 
@@ -664,6 +666,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
                              y.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), _stream(u))
     if rc:
         _abi.check(rc)
+    increment_version(out)
     return y, out
 
 

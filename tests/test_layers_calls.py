@@ -129,3 +129,26 @@ def test_steps_refuse_traces(op):
     x = torch.randn(2, 5, 8, device="cuda")
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(all_calls(x)[op], x)
+
+
+# ---- states written in place -----------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("inference", [False, True])
+def test_steps_count_as_writes_to_their_state(inference):
+    x = torch.randn(2, 5, 8, device="cuda")
+    w, A, B = parameters(x)
+    with torch.inference_mode(inference):
+        states = [torch.zeros(2, 3, 8, device="cuda"), torch.zeros(2, 8, 4, device="cuda")]
+        others = [torch.zeros_like(s) for s in states]
+        for out in (states, others):
+            basalto.causal_conv_step(x[:, 0], states[0], w, out_state=out[0])
+            basalto.selective_scan_step(x[:, 0], x[:, 0], A, B[:, 0], B[:, 0], states[1], out_state=out[1])
+    if not inference:
+        assert [s._version for s in states + others] == [1] * 4
+        # A state that a differentiable call has kept for its gradients is not written unnoticed.
+        leaf = w.clone().requires_grad_()
+        y = basalto.causal_conv(x, leaf, initial_state=states[0])
+        with torch.no_grad():
+            basalto.causal_conv_step(x[:, 0], states[0], w)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
