@@ -67,7 +67,12 @@ int occupancy(const void* fn, int threads, int smem) {
   auto it = cache.find(key);
   if (it != cache.end()) return it->second;
   int n = 0;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+  // Raised where it is too low, never lowered: another thread may be about to launch with more.
+  cudaFuncAttributes now;
+  if (cudaFuncGetAttributes(&now, fn) != cudaSuccess) return 0;
+  if (now.maxDynamicSharedSizeBytes < smem &&
+      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, threads, smem) != cudaSuccess) return 0;
   cache[key] = n;
   return n;

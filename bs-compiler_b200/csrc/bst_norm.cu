@@ -490,14 +490,17 @@ static int norm_launch(const NormArgs& a, int tpr, int64_t blocks, cudaStream_t 
     NormArgs args = a;
     args.stages = std::max(2, std::min(kNormMaxStages, 64 * 1024 / stage));
     const int smem = V > 1 ? kNormRingHeader + args.stages * stage : 0;
+    // The limit belongs to the kernel, not to the call: every call sets the same one, the most that any needs, so that
+    // calls with other row lengths on other threads cannot take this one's room away before its launch.
+    const int most_smem = V > 1 ? kNormRingHeader + kNormRingMost : 0;
     if constexpr (BWD) {
       auto* kernel = norm_backward_kernel<T, TPR, V>;
-      BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem));
       kernel<<<unsigned(blocks), NT, smem, st>>>(args);
     } else {
       // A block walks over the rows and keeps its parameters: no more of them than are resident.
       auto* kernel = norm_forward_kernel<T, TPR, V>;
-      BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      BST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem));
       const int64_t most = int64_t(sm_count()) * std::max(1, occupancy((const void*)kernel, NT, smem));
       kernel<<<unsigned(std::min(blocks, most)), NT, smem, st>>>(args);
     }

@@ -1,9 +1,12 @@
 """Calls of the layer operators around their kernels: streams, traces, forward-mode derivatives, version counters."""
+import ctypes
+import threading
+
 import pytest
 import torch
 
 import basalto
-from basalto import layers
+from basalto import _abi, layers
 
 
 def strided_lengths(values, device="cpu"):
@@ -152,3 +155,43 @@ def test_steps_count_as_writes_to_their_state(inference):
             basalto.causal_conv_step(x[:, 0], states[0], w)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+# ---- C callers on several threads --------------------------------------------------------------------
+@pytest.mark.gpu
+def test_c_calls_on_two_threads():
+    """Rows of two lengths through the same kernels, which need different amounts of shared memory (ctypes lets the
+    calls run at the same time)."""
+    lib, rows, dims = _abi.lib(), 4, (12000, 8200)
+
+    def caller(dim, failures):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            x, dy = torch.randn(2, rows, dim, device="cuda").unbind()
+            y, dx = torch.empty_like(x), torch.empty_like(x)
+            mean, rstd = torch.empty(2, rows, device="cuda").unbind()
+        d = _abi.CNormDesc(dtype=_abi.BST_F32, param_dtype=_abi.BST_F32, rows=rows, dim=dim, x_row=dim, y_row=dim,
+                           dy_row=dim, dx_row=dim, eps=1e-5)
+        p = [ctypes.c_void_p(t.data_ptr()) for t in (x, y, mean, rstd, dy, dx)]
+        st = ctypes.c_void_p(stream.cuda_stream)
+        for _ in range(2000):
+            rc = lib.bst_layer_norm_forward(ctypes.byref(d), p[0], None, None, p[1], p[2], p[3], st)
+            rc = rc or lib.bst_layer_norm_backward(ctypes.byref(d), p[0], None, p[4], p[2], p[3], p[5], None, None, None,
+                                                   0, st)
+            if rc:
+                failures.append((dim, rc, lib.bst_last_error()))
+                break
+        stream.synchronize()
+        want = torch.nn.functional.layer_norm(x.double(), (dim,))
+        # the mean's and the variance's sums (12 terms in a row, 10 levels), a root, a division: 64 half steps of
+        # values to 6
+        if not failures and (y - want).abs().max() > 6 * 64 * 2.0 ** -24:
+            failures.append((dim, "wrong values"))
+
+    failures = []
+    threads = [threading.Thread(target=caller, args=(dim, failures)) for dim in dims]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
