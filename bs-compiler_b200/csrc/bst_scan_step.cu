@@ -2,10 +2,13 @@
 //
 //   h' = exp(d A) h + d u B,   y = (sum_n C h' + D u) silu(z)
 // The state is read and written once in fp32 (8 bytes per entry) and dwarfs everything else, so HBM
-// bounds it; with a few sequences the launch does (256 x 4096 x 16 in bf16: 36 us on B200 for 143 MB, 3.9 TB/s of
+// bounds it; with a few sequences the launch does (256 x 4096 x 16 in bf16: 37 us on B200 for 143 MB, 3.8 TB/s of
 // a plain copy's 6.55; 2 x 1030 x 24 in fp32: 2.2 us).  L lanes share a channel, each with vectors of V
-// states, and reduce y over themselves; a thread has read its states before it writes them, so that
-// out_state may be the state itself.
+// states, and reduce y over themselves.  A thread has read its states before it writes them, so that
+// out_state may be the state itself.  The new state is computed as the scan's forward kernel does it, bit for
+// bit (the same decay, near 1 by its series: a sequence of tokens gathers its errors as a sequence of positions
+// does).  The series took 4 us at 256 x 4096 x 16; the work on step size and gate once per channel, not once
+// per lane, gave them back.
 #include <algorithm>
 
 #include "bst_scan.cuh"
@@ -38,7 +41,10 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const StepArgs a) {
   const bool in = i < a.channels;
   const int c = in ? i : 0, g = c / a.per_group;
   const int64_t b0 = int64_t(blockIdx.y) * NB;
-  float hv[NB][K][V], Av[K][V], raw[NB], u[NB], z[NB];
+  // What a sequence's lanes share (step size, gate, the sum's end) is one lane's work: lane l has OWN of the sequences.
+  constexpr int OWN = NB > L ? NB / L : 1;
+  const int own = NB == 1 ? 0 : l * OWN % NB;
+  float hv[NB][K][V], Av[K][V], d[OWN], du[OWN], u[OWN], z[OWN];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int n = (k * L + l) * V;
@@ -49,21 +55,29 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const StepArgs a) {
   }
   const float bias = a.dbias ? a.dbias[c] : 0.f, skip = a.D ? a.D[c] : 0.f;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int64_t b = b0 + j < a.batch ? b0 + j : 0;
-    raw[j] = to_f(static_cast<const T*>(a.delta)[b * a.db + c]);
-    u[j] = to_f(static_cast<const T*>(a.u)[b * a.ub + c]);
-    z[j] = a.z ? to_f(static_cast<const T*>(a.z)[b * a.zb + c]) : 0.f;
+  for (int i = 0; i < OWN; ++i) {
+    const int64_t b = b0 + own + i < a.batch ? b0 + own + i : 0;
+    d[i] = to_f(static_cast<const T*>(a.delta)[b * a.db + c]);
+    u[i] = to_f(static_cast<const T*>(a.u)[b * a.ub + c]);
+    z[i] = a.z ? to_f(static_cast<const T*>(a.z)[b * a.zb + c]) : 0.f;
   }
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    d[i] = a.softplus ? softplus(d[i] + bias) : d[i] + bias;
+    du[i] = d[i] * u[i];
+  }
+  const int lane = threadIdx.x % 32;
+  float y[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) y[j] = 0.f;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     if (b0 + j >= a.batch) break;
     const int64_t b = b0 + j;
-    const float d = a.softplus ? softplus(raw[j] + bias) : raw[j] + bias;
-    const float du = d * u[j], d2 = d * kLog2e;
+    const float dj = NB == 1 ? d[0] : __shfl_sync(0xffffffffu, d[j % OWN], lane - l + j / OWN);
+    const float duj = NB == 1 ? du[0] : __shfl_sync(0xffffffffu, du[j % OWN], lane - l + j / OWN);
     const T* B = static_cast<const T*>(a.B) + b * a.Bb + g * a.Bg;
     const T* C = static_cast<const T*>(a.C) + b * a.Cb + g * a.Cg;
-    float y = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int n = (k * L + l) * V;
@@ -72,21 +86,35 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const StepArgs a) {
         load_floats<T, V>(B + n, Bv);
         load_floats<T, V>(C + n, Cv);
         Chunk<float, V> o;
+        float e[V + V % 2];  // in pairs
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+          const float2 a2 = make_float2(Av[k][v] * kLog2e, Av[k][V == 1 ? 0 : v + 1] * kLog2e);
+          const float2 q = decay(both(dj), a2);
+          e[v] = q.x, e[v + 1] = q.y;
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          o.v[v] = fmaf(ex2(d2 * Av[k][v]), hv[j][k][v], du * Bv[v]);
-          y = fmaf(o.v[v], Cv[v], y);
+          o.v[v] = fmaf(e[v], hv[j][k][v], duj * Bv[v]);
+          y[j] = fmaf(o.v[v], Cv[v], y[j]);
         }
         if (in) *reinterpret_cast<Chunk<float, V>*>(a.out + b * a.ob + c * a.oc + n) = o;
       }
     }
+  }
+  constexpr int SPLIT = NB < L ? NB : L;  // lanes that end with sums of their own
 #pragma unroll
-    for (int m = L / 2; m >= 1; m >>= 1) y += __shfl_xor_sync(0xffffffffu, y, m);
-    if (in && l == 0) {
-      y = fmaf(skip, u[j], y);
-      if (a.z) y *= z[j] * sigmoid(z[j]);
-      static_cast<T*>(a.y)[b * a.yb + c] = from_f<T>(y);
-    }
+  for (int m = L / 2; m >= SPLIT; m >>= 1)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) y[j] += __shfl_xor_sync(0xffffffffu, y[j], m);
+  reduce_scatter<NB, SPLIT, 1>(y, lane);
+  if (!in || l >= SPLIT) return;
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const int64_t b = b0 + own + i;
+    float v = fmaf(skip, u[i], y[i]);
+    if (a.z) v *= z[i] * sigmoid(z[i]);
+    if (b < a.batch) static_cast<T*>(a.y)[b * a.yb + c] = from_f<T>(v);
   }
 }
 
@@ -128,7 +156,8 @@ extern "C" int bst_scan_step(const bst_scan_desc* d, const void* u, const void* 
         scan_step_kernel<T, L, V, K, NB><<<dim3(unsigned(cols), unsigned(turns)), 256, 0, st>>>(a);
         return launched("scan_step_kernel launch");
       };
-      if (K <= 2 && cols * ((d->batch + 3) / 4) >= int64_t(sm_count()) * 16) return launch(integral_constant<int, 4>{});
+      if constexpr (K <= 2)
+        if (cols * ((d->batch + 3) / 4) >= int64_t(sm_count()) * 16) return launch(integral_constant<int, 4>{});
       return launch(integral_constant<int, 1>{});
     };
     integral_constant<int, 1> one;
