@@ -128,6 +128,8 @@ def _recorded(name, stream, *ts):
 
 def _on(stream, fn, *args):
     """fn(*args) with `stream` current; the caching allocator learns that the inputs are used there."""
+    if stream.device != args[0].device:  # the kernels would run on another stream, unordered with this one
+        raise RuntimeError(f"basalto.{fn.__name__}: stream= is on {stream.device}, the input on {args[0].device}")
     with torch.cuda.stream(stream):
         out = fn(*args)
     for t in args:

@@ -1,6 +1,7 @@
 """Calls of the layer operators around their kernels: streams, traces, forward-mode derivatives, version counters."""
 import ctypes
 import threading
+import types
 
 import pytest
 import torch
@@ -64,6 +65,21 @@ def test_strided_lengths_in_compiled_graphs():
     grads = [torch.autograd.grad(sum(y.sum() for y in r), x)[0] for r in (got, want)]
     for a, b in zip([*got, grads[0]], [*want, grads[1]]):
         assert torch.equal(a, b)
+
+
+def test_streams_of_other_devices_are_refused(monkeypatch):
+    """The launch goes to the input's device: with another device's stream it would not run on that stream."""
+    monkeypatch.setattr(layers, "_cuda", lambda *_: None)
+    x = torch.zeros(2, 5, 8)
+    other = types.SimpleNamespace(device=torch.device("cuda", 1))
+    w, A, B = parameters(x)
+    for call in (lambda: basalto.layer_norm(x, stream=other), lambda: basalto.causal_conv(x, w, stream=other),
+                 lambda: basalto.selective_scan(x, x, A, B, B, stream=other),
+                 lambda: basalto.causal_conv_step(x[:, 0], torch.zeros(2, 3, 8), w, stream=other),
+                 lambda: basalto.selective_scan_step(x[:, 0], x[:, 0], A, B[:, 0], B[:, 0], torch.zeros(2, 8, 4),
+                                                     stream=other)):
+        with pytest.raises(RuntimeError, match="stream= is on cuda:1, the input on cpu"):
+            call()
 
 
 # ---- forward-mode derivatives and traces ----------------------------------------------------------
