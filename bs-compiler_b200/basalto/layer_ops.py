@@ -44,6 +44,7 @@ def _(dy, x, weight, mean, rstd, bias):
 def _norm_context(ctx, inputs, output):
     x, weight, bias, _ = inputs
     ctx.save_for_backward(x, weight, bias, output[1], output[2])
+    ctx.mark_non_differentiable(output[1], output[2])
 
 
 def _norm_grad(ctx, dy, _mean, _rstd):

@@ -211,3 +211,14 @@ def test_c_calls_on_two_threads():
     for t in threads:
         t.join()
     assert not failures
+
+
+# ---- custom operators called by their own names -------------------------------------------------------
+def test_statistics_of_the_norm_carry_no_gradient():
+    """torch.ops.basalto.layer_norm also returns mean and 1/std, whose gradients its backward pass does not have:
+    a loss on them is refused instead of getting zeros."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(2, 5, 8, device="cuda", requires_grad=True)
+        y, mean, rstd = torch.ops.basalto.layer_norm(x, None, None, 1e-5)
+        assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
