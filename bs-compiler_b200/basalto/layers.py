@@ -204,22 +204,25 @@ class _Norm(torch.autograd.Function):
         return (*_norm_backward(dy, x, weight, mean, rstd, ctx.bias_dtype, want_w, want_b), None)
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5, stream=None):
-    """Layer norm over the last axis of x.  weight, bias: [dim], of x's type or float32 (both of one type).
-
-    Statistics and arithmetic are float32 whatever the type; the biased variance is taken around the mean, in
-    a second sweep.  Rows may lie at any distance; other layouts are copied first."""
-    name = "layer_norm"
+def _norm_args(name, x, weight, bias, eps):
     _type(name, x)
     if x.dim() < 1:
         raise ValueError("basalto.layer_norm needs at least one axis")
-    eps = float(eps)
     if not eps >= 0:
         raise ValueError("basalto.layer_norm: eps must be non-negative")
     for what, p in (("weight", weight), ("bias", bias)):
         if p is not None:
             _param(name, what, p, (x.shape[-1],), x)
     _same_params(name, weight, bias)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, stream=None):
+    """Layer norm over the last axis of x.  weight, bias: [dim], of x's type or float32 (both of one type).
+
+    Statistics and arithmetic are float32 whatever the type; the biased variance is taken around the mean, in
+    a second sweep.  Rows may lie at any distance; other layouts are copied first."""
+    name, eps = "layer_norm", float(eps)
+    _norm_args(name, x, weight, bias, eps)
     if _recorded(name, stream, x, weight, bias):
         return torch.ops.basalto.layer_norm(x, weight, bias, eps)[0]
     _cuda(name, x)
@@ -340,6 +343,18 @@ def _conv_args(name, x, weight, bias, activation):
     return 1 if activation else 0
 
 
+def _conv_sequence_args(name, x, weight, bias, activation, initial_state, lengths):
+    _type(name, x)
+    if x.dim() != 3:
+        raise ValueError(f"basalto.causal_conv: x must be [batch, length, channels], got {tuple(x.shape)}")
+    silu = _conv_args(name, x, weight, bias, activation)
+    b, _, c = x.shape
+    if initial_state is not None:
+        _need(name, "initial_state", initial_state, (b, weight.shape[1] - 1, c), x.dtype, x.device)
+    _lengths(name, lengths, b, x.device)
+    return silu
+
+
 def causal_conv(x, weight, bias=None, activation=None, initial_state=None, lengths=None, return_state=False,
                 stream=None):
     """Causal depthwise convolution y[b, t, c] = act(bias[c] + sum_k weight[c, k] x[b, t - width + 1 + k, c]).
@@ -353,14 +368,7 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, lengt
     return_state: also return the last width - 1 inputs before each sequence's end, for the next piece of the
     sequence or for causal_conv_step."""
     name = "causal_conv"
-    _type(name, x)
-    if x.dim() != 3:
-        raise ValueError(f"basalto.causal_conv: x must be [batch, length, channels], got {tuple(x.shape)}")
-    silu = _conv_args(name, x, weight, bias, activation)
-    b, _, c = x.shape
-    if initial_state is not None:
-        _need(name, "initial_state", initial_state, (b, weight.shape[1] - 1, c), x.dtype, x.device)
-    _lengths(name, lengths, b, x.device)
+    silu = _conv_sequence_args(name, x, weight, bias, activation, initial_state, lengths)
     if _recorded(name, stream, x, weight, bias, initial_state):
         y, final = torch.ops.basalto.causal_conv(x, weight, bias, bool(silu), initial_state, lengths)
         return (y, final) if return_state else y
@@ -585,6 +593,18 @@ def _scan_args(name, u, delta, A, B, C, D, z, delta_bias):
     return B, C
 
 
+def _scan_sequence_args(name, u, delta, A, B, C, D, z, delta_bias, initial_state, lengths):
+    _type(name, u)
+    if u.dim() != 3:
+        raise ValueError(f"basalto.selective_scan: u must be [batch, length, channels], got {tuple(u.shape)}")
+    B, C = _scan_args(name, u, delta, A, B, C, D, z, delta_bias)
+    b, _, c = u.shape
+    if initial_state is not None:
+        _need(name, "initial_state", initial_state, (b, c, A.shape[1]), torch.float32, u.device)
+    _lengths(name, lengths, b, u.device)
+    return B, C
+
+
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False, initial_state=None,
                    lengths=None, return_state=False, stream=None):
     """Selective state space scan, per batch entry and channel c with the states n:
@@ -601,14 +621,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     nothing is read there.  return_state: also return the state after each sequence's last position, float32
     [batch, channels, states], for the next piece of the sequence or for selective_scan_step."""
     name = "selective_scan"
-    _type(name, u)
-    if u.dim() != 3:
-        raise ValueError(f"basalto.selective_scan: u must be [batch, length, channels], got {tuple(u.shape)}")
-    B, C = _scan_args(name, u, delta, A, B, C, D, z, delta_bias)
-    b, _, c = u.shape
-    if initial_state is not None:
-        _need(name, "initial_state", initial_state, (b, c, A.shape[1]), torch.float32, u.device)
-    _lengths(name, lengths, b, u.device)
+    B, C = _scan_sequence_args(name, u, delta, A, B, C, D, z, delta_bias, initial_state, lengths)
     if _recorded(name, stream, u, delta, A, B, C, D, z, delta_bias, initial_state):
         # Dynamo makes another graph for inputs with gradients; a trace has to serve those too.
         save = not torch.compiler.is_compiling() or _wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state)

@@ -192,8 +192,8 @@ def test_c_calls_on_two_threads():
         st = ctypes.c_void_p(stream.cuda_stream)
         for _ in range(2000):
             rc = lib.bst_layer_norm_forward(ctypes.byref(d), p[0], None, None, p[1], p[2], p[3], st)
-            rc = rc or lib.bst_layer_norm_backward(ctypes.byref(d), p[0], None, p[4], p[2], p[3], p[5], None, None, None,
-                                                   0, st)
+            rc = rc or lib.bst_layer_norm_backward(ctypes.byref(d), p[0], None, p[4], p[2], p[3], p[5], None, None,
+                                                   None, 0, st)
             if rc:
                 failures.append((dim, rc, lib.bst_last_error()))
                 break
@@ -222,3 +222,52 @@ def test_statistics_of_the_norm_carry_no_gradient():
         x = torch.empty(2, 5, 8, device="cuda", requires_grad=True)
         y, mean, rstd = torch.ops.basalto.layer_norm(x, None, None, 1e-5)
         assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+
+
+@pytest.mark.parametrize("fake", [False, True])
+def test_custom_operators_check_their_arguments(fake):
+    """A wrong shape or type would be read out of range: refused before any launch, as by the functions."""
+    import contextlib
+
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    o = torch.ops.basalto
+    with FakeTensorMode() if fake else contextlib.nullcontext():
+        def t(*shape, dtype=torch.float32):
+            return torch.empty(shape, dtype=dtype, device="cuda" if fake else "cpu")
+
+        x, w, p, A, B, h = t(2, 5, 8), t(8, 4), t(8), t(8, 4), t(2, 5, 1, 4), t(2, 8, 4)
+        stat, saved, half = t(10), t(2 * 8 * 4 * 4, dtype=torch.uint8), torch.bfloat16
+        lens = t(2, dtype=torch.int64)
+
+        def conv(x=x, w=w, bias=None, initial=None, lengths=None):
+            return o.causal_conv(x, w, bias, True, initial, lengths)
+
+        def scan(u=x, delta=x, A=A, B=B, C=B, D=None, z=None, bias=None, initial=None, lengths=None):
+            return o.selective_scan(u, delta, A, B, C, D, z, bias, True, initial, lengths, True)
+
+        def scan_grad(dy=x, dfinal=h, u=x, delta=x, A=A, B=B, saved=saved, lengths=None):
+            return o.selective_scan_backward(dy, dfinal, u, delta, A, B, B, None, None, None, True, lengths, saved)
+
+        refused = [
+            lambda: o.layer_norm(x, t(7), None, 1e-5), lambda: o.layer_norm(x, p.to(half), None, 1e-5),
+            lambda: o.layer_norm(x, None, None, -1.0), lambda: o.layer_norm(x.double(), None, None, 1e-5),
+            lambda: o.layer_norm_backward(t(2, 5, 7), x, p, stat, stat, p),
+            lambda: o.layer_norm_backward(x.to(half), x, p, stat, stat, p),
+            lambda: o.layer_norm_backward(x, x, p, t(9), stat, p),
+            lambda: conv(w=t(7, 4)), lambda: conv(w=t(8, 9)), lambda: conv(bias=t(7)), lambda: conv(initial=t(2, 2, 8)),
+            lambda: conv(lengths=lens),
+            lambda: o.causal_conv_backward(t(2, 4, 8), t(2, 3, 8), x, w, None, True, None, None),
+            lambda: o.causal_conv_backward(x, t(2, 2, 8), x, w, None, True, None, None),
+            lambda: scan(delta=t(2, 5, 7)), lambda: scan(A=t(8, 65)), lambda: scan(B=t(2, 5, 4), C=t(2, 5, 4)),
+            lambda: scan(C=t(2, 5, 1, 3)), lambda: scan(D=t(7)), lambda: scan(z=t(2, 4, 8)), lambda: scan(bias=t(7)),
+            lambda: scan(initial=t(2, 8, 3)), lambda: scan(lengths=lens),
+            lambda: scan_grad(dy=t(2, 4, 8)), lambda: scan_grad(dfinal=t(2, 8, 3)), lambda: scan_grad(saved=saved[:-1]),
+            lambda: scan_grad(B=t(2, 4, 1, 4)), lambda: scan_grad(saved=t(0, dtype=torch.uint8)),
+        ]
+        for call in refused:
+            with pytest.raises((ValueError, TypeError)):
+                call()
+        if fake:
+            o.layer_norm_backward(x, x, p, stat, stat, p)
+            o.causal_conv_backward(x, t(2, 3, 8), x, w, None, True, None, None)
+            scan(), scan_grad()
