@@ -141,9 +141,11 @@ def _on(stream, fn, *args):
 # ---- layer norm ----------------------------------------------------------------------------
 def _rows(x):
     """x as [rows, dim] with contiguous rows at one distance (a copy where its strides do not allow it)."""
+    if not x.numel():
+        return x.reshape(0, x.shape[-1])
     if x.dim() != 2:
         try:
-            x = x.view(-1, x.shape[-1]) if x.numel() else x.reshape(0, x.shape[-1])
+            x = x.view(-1, x.shape[-1])
         except RuntimeError:
             x = x.contiguous().view(-1, x.shape[-1])
     return _dense(x)

@@ -271,3 +271,11 @@ def test_custom_operators_check_their_arguments(fake):
             o.layer_norm_backward(x, x, p, stat, stat, p)
             o.causal_conv_backward(x, t(2, 3, 8), x, w, None, True, None, None)
             scan(), scan_grad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 0), (0, 8), (2, 0, 8), (2, 3, 0), (5,)])
+def test_norm_of_empty_rows_has_the_shapes_of_its_fake(shape):
+    x = torch.randn(shape, device="cuda", requires_grad=True)
+    torch.library.opcheck(torch.ops.basalto.layer_norm.default, (x, None, None, 1e-5),
+                          test_utils=("test_schema", "test_faketensor"))
