@@ -2,12 +2,12 @@
 //
 //   h' = exp(d A) h + d u B,   y = (sum_n C h' + D u) silu(z)
 // The state is read and written once in fp32 (8 bytes per entry) and dwarfs everything else, so HBM
-// bounds it; with a few sequences the launch does (256 x 4096 x 16 in bf16: 37 us on B200 for 143 MB, 3.8 TB/s of
+// bounds it; with a few sequences the launch does (256 x 4096 x 16 in bf16: 33 us on B200 for 143 MB, 4.3 TB/s of
 // a plain copy's 6.55; 2 x 1030 x 24 in fp32: 2.2 us).  L lanes share a channel, each with vectors of V
 // states, and reduce y over themselves.  A thread has read its states before it writes them, so that
 // out_state may be the state itself.  The new state is computed as the scan's forward kernel does it, bit for
 // bit (the same decay, near 1 by its series: a sequence of tokens gathers its errors as a sequence of positions
-// does).  The series took 4 us at 256 x 4096 x 16; the work on step size and gate once per channel, not once
+// does).  The series took 4 us at 256 x 4096 x 16; the work on step size and gate done once per channel, not once
 // per lane, gave them back.
 #include <algorithm>
 
@@ -25,6 +25,10 @@ struct StepArgs {
   int channels, per_group, states, softplus;
 };
 
+// Small blocks start and end at different times, so that loads and stores overlap more (and a ninth fits the registers):
+// 33 us at 256 x 4096 x 16, with 256 threads 37.
+constexpr int kStepThreads = 128;
+
 template <typename T, int V>
 __device__ __forceinline__ void load_floats(const T* p, float (&v)[V]) {
   const Chunk<T, V> c = *reinterpret_cast<const Chunk<T, V>*>(p);
@@ -36,8 +40,8 @@ __device__ __forceinline__ void load_floats(const T* p, float (&v)[V]) {
 // per thread: what belongs to the channel (A, D, the step's bias) is read once for them, and their states are on
 // their way together.
 template <typename T, int L, int V, int K, int NB>
-__global__ void __launch_bounds__(256) scan_step_kernel(const StepArgs a) {
-  const int i = int(blockIdx.x) * (256 / L) + int(threadIdx.x) / L, l = threadIdx.x % L;
+__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const StepArgs a) {
+  const int i = int(blockIdx.x) * (kStepThreads / L) + int(threadIdx.x) / L, l = threadIdx.x % L;
   const bool in = i < a.channels;
   const int c = in ? i : 0, g = c / a.per_group;
   const int64_t b0 = int64_t(blockIdx.y) * NB;
@@ -144,20 +148,20 @@ extern "C" int bst_scan_step(const bst_scan_desc* d, const void* u, const void* 
   return with_type(d->dtype, [&](auto t) {
     using T = decltype(t);
     using std::integral_constant;
-    // Four sequences per thread where that leaves two full turns of blocks (256 x 4096 x 16: 57 us with one, 36 with
-    // four), one where threads are scarce.
+    // Four sequences per thread where that leaves two full turns of blocks (256 x 4096 x 16 in blocks of 256: 57 us
+    // with one, 36 with four), one where threads are scarce.
     auto go = [&](auto lc, auto vc, auto kc) {
       constexpr int L = decltype(lc)::value, V = decltype(vc)::value, K = decltype(kc)::value;
-      const int64_t cols = (d->channels * L + 255) / 256;
+      const int64_t cols = (d->channels * L + kStepThreads - 1) / kStepThreads;
       auto launch = [&](auto nb) {
         constexpr int NB = decltype(nb)::value;
         const int64_t turns = (d->batch + NB - 1) / NB;
         if (turns > 65535) return fail(BST_ERR_UNSUPPORTED, "the step takes up to 65535 sequences (more in large batches)");
-        scan_step_kernel<T, L, V, K, NB><<<dim3(unsigned(cols), unsigned(turns)), 256, 0, st>>>(a);
+        scan_step_kernel<T, L, V, K, NB><<<dim3(unsigned(cols), unsigned(turns)), kStepThreads, 0, st>>>(a);
         return launched("scan_step_kernel launch");
       };
       if constexpr (K <= 2)
-        if (cols * ((d->batch + 3) / 4) >= int64_t(sm_count()) * 16) return launch(integral_constant<int, 4>{});
+        if (cols * ((d->batch + 3) / 4) >= int64_t(sm_count()) * 32) return launch(integral_constant<int, 4>{});
       return launch(integral_constant<int, 1>{});
     };
     integral_constant<int, 1> one;
