@@ -149,7 +149,8 @@ def _causal_conv(n):
 # What may stand between a pattern's F.pad and its convolution: operations that write to nothing.
 _VIEWS = {"chunk", "contiguous", "detach", "expand", "permute", "reshape", "size", "split", "squeeze", "to", "transpose",
           "unsqueeze", "view"}
-_READERS = {operator.getitem, F.layer_norm, layers.layer_norm, conv_channels_first} | _PAD | _CONV
+_READERS = {operator.getitem, operator.add, operator.sub, operator.mul, operator.truediv, operator.neg, F.layer_norm,
+            layers.layer_norm, conv_channels_first} | _PAD | _CONV
 
 
 def _reads_only(n):

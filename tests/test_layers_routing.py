@@ -151,6 +151,12 @@ def test_several_convolutions_of_one_input(plain):
 
     same_effects(two, 3, x=x_(), w=torch.randn(C, 1, TAPS))
 
+    def scaled(x, w):
+        p = F.pad(x, (TAPS - 1, 0))
+        return F.conv1d(p, (w * 2 + 1).contiguous(), groups=C)
+
+    same_effects(scaled, 1, x=x_(), w=torch.randn(C, 1, TAPS))
+
 
 @pytest.mark.parametrize("write", [lambda x: x.mul_(2), lambda x: F.relu(x, inplace=True), lambda x: F.relu(x, True),
                                    lambda x: torch.add(x, 1, out=x), lambda x: x[0].zero_(), lambda x: torch.relu_(x),
