@@ -72,12 +72,17 @@ def _ptr(t):
 
 def _guard(t):
     """Makes the tensor's device current for the launch (nothing to do when it already is)."""
-    i = t.device.index
-    return _NO_GUARD if i == torch.cuda.current_device() else torch.cuda.device(i)
+    i = t.get_device()
+    return _NO_GUARD if i == torch._C._cuda_getDevice() else torch.cuda.device(i)
 
 
 def _stream(t):
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _empty(t):
+    """A new contiguous tensor like t (a third of the host time of torch.empty with t's shape, type and device)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _dense(t):
@@ -107,9 +112,10 @@ def _no_tangents(name, *ts):
 
 def _tracing():
     """Whether torch operators are being recorded (torch.jit.trace, make_fx): a launch would be missing there."""
-    if torch._C._get_tracing_state() is not None:
+    if torch._C._is_tracing():
         return True
-    if torch._C._len_torch_dispatch_stack() or torch._ops._len_torch_dispatch_stack_pre_dispatch():
+    # make_fx works through a dispatch mode, or before dispatch through a function mode.
+    if torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():
         from torch.fx.experimental.proxy_tensor import get_proxy_mode
         return get_proxy_mode() is not None
     return False
@@ -155,7 +161,7 @@ def _norm_forward(x, weight, bias, eps, stats):
     x2 = _rows(x)
     m, n = x2.shape
     p = weight if weight is not None else bias
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty(x)
     mean = rstd = None
     if stats:
         mean = torch.empty(m, dtype=torch.float32, device=x.device)
@@ -174,7 +180,7 @@ def _norm_backward(dy, x, weight, mean, rstd, bias_dtype, want_w, want_b):
     x2, g2 = _rows(x), _rows(dy)
     m, n = x2.shape
     pt = weight.dtype if weight is not None else (bias_dtype or x.dtype)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _empty(x)
     dw = torch.empty(n, dtype=pt, device=x.device) if want_w else None
     db = torch.empty(n, dtype=pt, device=x.device) if want_b else None
     code, pcode, dims = _DT[x.dtype], _DT[pt], (m, n, x2.stride(0), n, g2.stride(0), n)
@@ -263,7 +269,7 @@ def _conv_empty(x, lines, strides=None):
         return torch.empty_strided((b, n, c), strides, dtype=x.dtype, device=x.device)
     if lines:
         return torch.empty(b, c, n, dtype=x.dtype, device=x.device).transpose(1, 2)
-    return torch.empty(b, n, c, dtype=x.dtype, device=x.device)
+    return _empty(x)
 
 
 def _step_of(x, lines):
@@ -411,11 +417,14 @@ def _out_state(name, state, out_state):
     if out_state is None or out_state is state:
         return state
     _need(name, "out_state", out_state, state.shape, state.dtype, state.device)
-    if state.untyped_storage().data_ptr() != out_state.untyped_storage().data_ptr():
+    at, to = state.data_ptr(), out_state.data_ptr()
+    if at == to and state.stride() == out_state.stride():
         return out_state
-    if state.numel() and out_state.data_ptr() == state.data_ptr() and out_state.stride() == state.stride():
-        return out_state
-    if state.numel() and _spans_meet(state, out_state):
+    if state.is_contiguous() and out_state.is_contiguous():
+        meet = abs(at - to) < state.nbytes
+    else:
+        meet = state.numel() and _spans_meet(state, out_state)
+    if meet:
         raise ValueError(f"basalto.{name}: out_state overlaps state")
     return out_state
 
@@ -460,12 +469,12 @@ def causal_conv_step(x, state, weight, bias=None, activation=None, out_state=Non
     if stream is not None:
         return _on(stream, causal_conv_step, x, state, weight, bias, activation, out)
     for t in (state, out):
-        if t.numel() and ((c > 1 and t.stride(2) != 1) or (width > 2 and t.stride(1) != c)):
+        if not t.is_contiguous() and ((c > 1 and t.stride(2) != 1) or (width > 2 and t.stride(1) != c)):
             raise ValueError("basalto.causal_conv_step: the state's rows must be contiguous")
-    if b > 1:
+    if not out.is_contiguous():
         _distinct(name, "the state", out)
     x, weight, bias = _dense(x), weight.contiguous(), _dense(bias)
-    y = torch.empty(b, c, dtype=x.dtype, device=x.device)
+    y = _empty(x)
     with _guard(x):
         rc = _rust.causal_conv_step(code, _DT[weight.dtype], width, silu, b, c, x.stride(0), c, x.data_ptr(),
                                     state.data_ptr(), state.stride(0), weight.data_ptr(), _ptr(bias), y.data_ptr(),
@@ -504,7 +513,7 @@ def _scan_forward(u, delta, A, B, C, D, z, bias, softplus, initial, lengths, wan
     u, delta, z, B, C = _dense(u), _dense(delta), _dense(z), _dense(B), _dense(C)
     dev = u.device
     b, n, c = u.shape
-    y = torch.empty(b, n, c, dtype=u.dtype, device=dev)
+    y = _empty(u)
     final = torch.empty(b, c, A.shape[1], dtype=torch.float32, device=dev) if want_state else None
     head = _scan_head(u, delta, z, y, None, B, C, softplus)
     with _guard(u):
@@ -523,13 +532,11 @@ def _scan_backward(dy, dfinal, u, delta, A, B, C, D, z, bias, softplus, lengths,
     """(du, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dinitial)"""
     u, delta, z, B, C, dy = _dense(u), _dense(delta), _dense(z), _dense(B), _dense(C), _dense(dy)
     dfinal = None if dfinal is None else dfinal.contiguous()
-    dev, t = u.device, u.dtype
-    du, ddelta = torch.empty(u.shape, dtype=t, device=dev), torch.empty(u.shape, dtype=t, device=dev)
-    dB, dC = torch.empty(B.shape, dtype=t, device=dev), torch.empty(C.shape, dtype=t, device=dev)
-    dA = torch.empty(A.shape, dtype=torch.float32, device=dev)
-    dz = None if z is None else torch.empty(u.shape, dtype=t, device=dev)
-    dD = None if D is None else torch.empty(D.shape, dtype=torch.float32, device=dev)
-    dbias = None if bias is None else torch.empty(bias.shape, dtype=torch.float32, device=dev)
+    dev = u.device
+    du, ddelta, dA, dB, dC = _empty(u), _empty(u), _empty(A), _empty(B), _empty(C)
+    dz = None if z is None else _empty(u)
+    dD = None if D is None else _empty(D)
+    dbias = None if bias is None else _empty(bias)
     dinit = None
     if want_initial:
         dinit = torch.empty(u.shape[0], u.shape[2], A.shape[1], dtype=torch.float32, device=dev)
@@ -673,7 +680,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
         _distinct(name, "the state", out)
     u, delta, z, B, C = _dense(u), _dense(delta), _dense(z), _dense(B), _dense(C)
     A, D, delta_bias = A.contiguous(), _dense(D), _dense(delta_bias)
-    y = torch.empty(b, c, dtype=u.dtype, device=u.device)
+    y = _empty(u)
     with _guard(u):
         (Bb, Bg, _), (Cb, Cg, _) = B.stride(), C.stride()
         rc = _rust.scan_step(code, 1 if delta_softplus else 0, b, c, n, B.shape[1], u.stride(0), delta.stride(0),
