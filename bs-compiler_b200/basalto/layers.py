@@ -87,7 +87,9 @@ def _empty(t):
 
 def _dense(t):
     """`t`, or a copy of it, with its last axis contiguous."""
-    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    if t is None or t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] <= 1:
+        return t
+    return t.contiguous()
 
 
 def _lengths(name, lengths, batch, device):
