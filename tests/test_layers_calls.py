@@ -279,3 +279,21 @@ def test_norm_of_empty_rows_has_the_shapes_of_its_fake(shape):
     x = torch.randn(shape, device="cuda", requires_grad=True)
     torch.library.opcheck(torch.ops.basalto.layer_norm.default, (x, None, None, 1e-5),
                           test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.gpu
+def test_compiled_graphs_of_changing_lengths():
+    """One graph for every length and batch (symbolic sizes), with gradients."""
+    def f(x, w, A, B, lengths):
+        v = basalto.causal_conv(basalto.layer_norm(x), w, activation="silu", lengths=lengths)
+        return basalto.selective_scan(v, x, A, B, B, delta_softplus=True, lengths=lengths)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend="basalto", fullgraph=True, dynamic=True)
+    for batch, length in ((2, 40), (3, 17), (5, 64)):
+        x = torch.randn(batch, length, 16, device="cuda", requires_grad=True)
+        w, A, B = parameters(x)
+        lengths = torch.full((batch,), length - 3, dtype=torch.int32, device="cuda")
+        y, want = compiled(x, w, A, B, lengths), f(x, w, A, B, lengths)
+        assert torch.equal(y, want)
+        assert torch.equal(torch.autograd.grad(y.sum(), x)[0], torch.autograd.grad(want.sum(), x)[0])
