@@ -7,8 +7,10 @@
   by taps - 1 on both sides and cut back to the sequence ([..., :length]), or over an F.pad(x, (taps - 1, 0)) of
   zeros; a silu of the result that nothing else reads goes into the same kernel.
 
-It replaces them and returns how many it replaced.  Their gradients are the kernels' own.  Shapes and types are
-those of Dynamo's example values; nodes without them, or with symbolic sizes, are left alone.
+It replaces them and returns how many it replaced.  Their gradients are the kernels' own.  Shapes, types and strides
+are those of Dynamo's example values; nodes without them, or with symbolic sizes, are left alone.  No other node is
+removed, a replacement stands where the layer norm or the convolution stood, and a pad is read through only if nothing
+can write to its source: in-place operations of the graph keep their effect and their order.
 `has_layer_ops(gm)`: whether the user's code itself called one of the custom operators torch.ops.basalto.*.
 """
 from __future__ import annotations
