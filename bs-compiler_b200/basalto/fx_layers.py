@@ -153,6 +153,9 @@ _VIEWS = {"chunk", "contiguous", "detach", "expand", "permute", "reshape", "size
           "unsqueeze", "view"}
 _READERS = {operator.getitem, operator.add, operator.sub, operator.mul, operator.truediv, operator.neg, F.layer_norm,
             layers.layer_norm, conv_channels_first} | _PAD | _CONV
+# Python's operators that write in place.
+_WRITERS = {"setitem", "delitem", "iadd", "iand", "iconcat", "ifloordiv", "ilshift", "imatmul", "imod", "imul", "ior",
+            "ipow", "irshift", "isub", "itruediv", "ixor"}
 
 
 def _reads_only(n):
@@ -171,11 +174,11 @@ def _writes_to(n, value):
     elif isinstance(n.target, torch._ops.OpOverload):
         writes = n.target._schema.is_mutable
     elif module in ("_operator", "operator"):
-        writes = name in ("setitem", "delitem") or hasattr(operator, f"__{name}__") and name[0] == "i" and \
-            hasattr(operator, name[1:].rstrip("_"))
+        writes = name in _WRITERS
     else:
-        writes = name.endswith("_") or n.op != "call_function" or not (module.startswith("torch") or
-                                                                       hasattr(torch, name))
+        own = not isinstance(n.target, torch._ops.HigherOrderOperator) and (module.startswith("torch") or
+                                                                            hasattr(torch, name))
+        writes = name.endswith("_") or n.op != "call_function" or not own
     if not (writes or n.kwargs.get("out") is not None or n.kwargs.get("inplace") or any(a is True for a in n.args[1:])):
         return False
     memory = value.untyped_storage()._cdata

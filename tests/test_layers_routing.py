@@ -2,6 +2,8 @@
 
 The routed graphs run here on the CPU, with plain torch in place of the two kernels.
 """
+import operator
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -161,7 +163,8 @@ def test_several_convolutions_of_one_input(plain):
 @pytest.mark.parametrize("write", [lambda x: x.mul_(2), lambda x: F.relu(x, inplace=True), lambda x: F.relu(x, True),
                                    lambda x: torch.add(x, 1, out=x), lambda x: x[0].zero_(), lambda x: torch.relu_(x),
                                    lambda x: x.__setitem__(0, 1.0), lambda x: x.__iadd__(1),
-                                   lambda x: torch.ops.aten.mul_.Tensor(x, x)])
+                                   lambda x: torch.ops.aten.mul_.Tensor(x, x), lambda x: operator.imul(x, 2),
+                                   lambda x: torch.ops.aten.add.out(x, x, out=x)])
 def test_a_pad_whose_source_is_written_later_stays_for_the_gradients(write):
     """The kernel keeps the source for its gradients, the padded convolution its copy."""
     w = torch.randn(C, 1, TAPS)
